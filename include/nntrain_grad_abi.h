@@ -43,6 +43,23 @@ typedef struct nntrain_native_error_info {
     uint32_t reserved;
 } nntrain_native_error_info;
 
+/* One tensor of a gradient list (ABI minor 36; no counterpart in the
+ * reference, which passes one tensor per call).  kind: 0 = fp32, 1 = bf16,
+ * 2 = BFP8.  values: the tensor, or its payload.  scales, block_size: of a
+ * BFP8 tensor (block_size 0 = one scale).  destination: where the clipped
+ * values (of a BFP8 tensor: the clipped scales) go, NULL = in place; it may
+ * not overlap `values` in part.  Addresses need the alignment of their type
+ * only.  first_chunk is filled in by nntrain_gradient_list_plan. */
+typedef struct nntrain_gradient_tensor {
+    const void* values;
+    float* scales;
+    void* destination;
+    int64_t length;
+    int64_t first_chunk;
+    int32_t kind;
+    int32_t block_size;
+} nntrain_gradient_tensor;
+
 /* ---- process-level ------------------------------------------------------ */
 
 /* (major << 16) | minor; major 1, minor 36.
@@ -283,6 +300,32 @@ int nntrain_gradient_clip_coefficient(int device, const double* squared_sum, flo
  * nntrain_gradient_clip_coefficient) and a value of exactly 1 touches nothing. */
 int nntrain_gradient_clip_apply(int device, int kind, void* values, long long count, float multiplier,
                                 const float* coefficient, nntrain_stream_t stream);
+
+/* ABI minor 36.  Host only: cuts a list into the chunks its kernels work on.
+ * Fills tensors[i].first_chunk and, when chunk_map is not null, 2 words per
+ * chunk (tensor, index in the tensor); chunk_values is the length of a chunk.
+ * Call it with a null chunk_map for the count, then with room for `capacity`
+ * chunks; copy table and map to the device and use them for as long as
+ * addresses and lengths stay what they are. */
+int nntrain_gradient_list_plan(nntrain_gradient_tensor* tensors, int count, int* chunk_map,
+                               long long capacity, long long* chunk_count, int* chunk_values);
+/* ABI minor 36.  The global norm over a list of tensors of mixed kinds and the
+ * clip, without a host read between them (the reference launches per tensor and
+ * reads the sum back: NNtrain.Core/Tensors/Tensor.CudaKernels.cs:119-854,
+ * NNtrain.Core/Torch/nn.cs:32-81).  tensors, chunk_map: the planned list, on
+ * the device.  workspace: chunk_count doubles that calls in flight at the same
+ * time do not share.  norm_and_coefficient as in
+ * nntrain_gradient_clip_coefficient; tensor_norms (optional): one fp32 norm per
+ * tensor.  apply != 0: destination = value * coefficient (bf16 rounded once;
+ * BFP8: scale = fmaxf(scale * coefficient, FLT_MIN), payload untouched); a
+ * coefficient of 1 copies, and leaves alone what is clipped in place.  A norm
+ * that is not finite (a NaN / Inf value, a BFP8 scale that is not finite and
+ * positive) sets *finite_status (optional) to 1 and gives the coefficient 1.
+ * Sums are binary64 in a fixed order: same list, same bits. */
+int nntrain_gradient_list_clip(
+    int device, const nntrain_gradient_tensor* tensors, int count, const int* chunk_map,
+    long long chunk_count, int chunk_values, double* workspace, float max_norm, int apply,
+    float* norm_and_coefficient, float* tensor_norms, int* finite_status, nntrain_stream_t stream);
 
 /* ABI minor 36.  AdamW that reads the reduced BFP8 gradient directly: the
  * arithmetic of the reference's adamw_kernel (NNtrain.Cuda/native/

@@ -1,0 +1,427 @@
+// Global L2 norm over a list of separately allocated gradient tensors, and the
+// clip that follows from it (ABI minor 36).
+//
+// The reference walks the leaves: one sum-of-squares launch and one scale
+// launch per tensor with a host read between them (NNtrain.Core/Tensors/
+// Tensor.CudaKernels.cs:119-854, NNtrain.Core/Torch/nn.cs:32-81).  Here a table
+// of the tensors lies on the device and three launches serve all of them:
+//
+//   squares   one CTA per chunk of a tensor -> one binary64 partial per chunk
+//   finish    one CTA: partials -> tensor norms -> norm and coefficient
+//   clip      one CTA per chunk again: destination = value * coefficient
+//
+//   n_t = sqrt(sum of v^2),  n = (float)sqrt(sum of n_t^2),
+//   c   = n > max_norm ? max_norm / (n + 1e-6f) : 1
+//
+// Every sum is binary64 in a fixed order (no atomics), so the same list gives
+// the same bits every time.  Squares of BFP8 values are summed as integers:
+// sum over blocks of scale^2 * (sum of code^2), the inner sum exact, which
+// keeps the fp32 -> fp64 conversions (16 per clock and SM) off the path.
+// A norm that is not finite in binary32 raises the flag and gives c = 1, so a
+// list that holds a NaN or an Inf comes out as it went in.
+//
+// Bound: HBM.  The norm has to be known before the first value is written, so
+// values are read twice; the clip walks the chunks from the back, where the
+// values that the squares pass read last are still in L2 (126 MB).
+#include "operator_launch.cuh"
+
+#include "nntrain_grad_abi.h"
+
+namespace ngb {
+namespace {
+
+enum TensorKind : int { kKindF32 = 0, kKindBf16 = 1, kKindBfp8 = 2 };
+
+constexpr int kUnroll = 4;              // 128-bit loads in flight per thread
+constexpr int kFinishThreads = 1024;
+
+// A chunk is 4096 values at least (one trip of a CTA over fp32) and grows with
+// the list so that the finish kernel, one CTA, has at most about 64 Ki
+// partials; 65536 at most, so that the last wave of CTAs stays short.
+constexpr long long kChunkLeast = 4096, kChunkMost = 65536;
+
+struct alignas(8) Chunk {
+    int tensor;
+    unsigned index;                     // values [index, index + 1) * chunk_values of the tensor
+};
+
+__device__ __forceinline__ double square_of(float v) {
+    const double d = static_cast<double>(v);
+    return d * d;
+}
+
+// The unaligned head of a range that starts at `p`: values before the first
+// 16-byte boundary (values are at least as aligned as their type).
+__device__ __forceinline__ int head_values(const void* p, int value_bytes, int n) {
+    const int head = static_cast<int>((16u - (static_cast<unsigned>(reinterpret_cast<std::uintptr_t>(p)) & 15u)) & 15u) / value_bytes;
+    return head < n ? head : n;
+}
+
+__device__ double chunk_squares_f32(const float* p, int n) {
+    const int head = head_values(p, 4, n), vectors = (n - head) >> 2, tail = head + vectors * 4;
+    double a = 0.0, b = 0.0;
+    if (static_cast<int>(threadIdx.x) < head) a += square_of(p[threadIdx.x]);
+    if (tail + static_cast<int>(threadIdx.x) < n) b += square_of(p[tail + threadIdx.x]);
+    const float4* body = reinterpret_cast<const float4*>(p + head);
+    int i = threadIdx.x;
+    for (; i + (kUnroll - 1) * kThreads < vectors; i += kUnroll * kThreads) {
+        float4 x[kUnroll];
+        #pragma unroll
+        for (int j = 0; j < kUnroll; ++j) x[j] = __ldg(body + i + j * kThreads);
+        #pragma unroll
+        for (int j = 0; j < kUnroll; ++j) {
+            a += square_of(x[j].x); b += square_of(x[j].y);
+            a += square_of(x[j].z); b += square_of(x[j].w);
+        }
+    }
+    for (; i < vectors; i += kThreads) {
+        const float4 x = __ldg(body + i);
+        a += square_of(x.x); b += square_of(x.y);
+        a += square_of(x.z); b += square_of(x.w);
+    }
+    return a + b;
+}
+
+__device__ double chunk_squares_bf16(const unsigned short* p, int n) {
+    const int head = head_values(p, 2, n), vectors = (n - head) >> 3, tail = head + vectors * 8;
+    double a = 0.0, b = 0.0;
+    if (static_cast<int>(threadIdx.x) < head) a += square_of(bf16_value(p[threadIdx.x]));
+    if (tail + static_cast<int>(threadIdx.x) < n) b += square_of(bf16_value(p[tail + threadIdx.x]));
+    const uint4* body = reinterpret_cast<const uint4*>(p + head);
+    int i = threadIdx.x;
+    for (; i + (kUnroll - 1) * kThreads < vectors; i += kUnroll * kThreads) {
+        uint4 x[kUnroll];
+        #pragma unroll
+        for (int j = 0; j < kUnroll; ++j) x[j] = __ldg(body + i + j * kThreads);
+        #pragma unroll
+        for (int j = 0; j < kUnroll; ++j) {
+            a += square_of(bf16_low(x[j].x)); b += square_of(bf16_high(x[j].x));
+            a += square_of(bf16_low(x[j].y)); b += square_of(bf16_high(x[j].y));
+            a += square_of(bf16_low(x[j].z)); b += square_of(bf16_high(x[j].z));
+            a += square_of(bf16_low(x[j].w)); b += square_of(bf16_high(x[j].w));
+        }
+    }
+    for (; i < vectors; i += kThreads) {
+        const uint4 x = __ldg(body + i);
+        a += square_of(bf16_low(x.x)); b += square_of(bf16_high(x.x));
+        a += square_of(bf16_low(x.y)); b += square_of(bf16_high(x.y));
+        a += square_of(bf16_low(x.z)); b += square_of(bf16_high(x.z));
+        a += square_of(bf16_low(x.w)); b += square_of(bf16_high(x.w));
+    }
+    return a + b;
+}
+
+// scale^2, or NaN for a scale that no encoding has (NaN, Inf, zero, negative):
+// such a tensor makes the norm NaN, which raises the flag.
+__device__ __forceinline__ double scale_square(float scale) {
+    if (!(scale > 0.0f) || is_non_finite(scale)) return __longlong_as_double(0x7ff8000000000000ll);
+    return square_of(scale);
+}
+
+// Codes [start, start + n) of a payload whose blocks of `block` values begin at
+// its first value.  A 16-byte word lies inside one block when block % 16 == 0
+// (or there is one block only) and the payload is 16-byte aligned; chunks start
+// at multiples of 4096 values.  Other layouts go value by value.
+__device__ double chunk_squares_bfp8(const signed char* payload, const float* scales, long long start, int n,
+                                     long long block, bool one_block) {
+    double a = 0.0;
+    const bool vector_ok = (reinterpret_cast<std::uintptr_t>(payload) & 15u) == 0 && (one_block || block % 16 == 0);
+    const int vectors = vector_ok ? n >> 4 : 0;
+    const uint4* body = reinterpret_cast<const uint4*>(payload + start);
+    for (int i = threadIdx.x; i < vectors; i += kThreads) {
+        const uint4 w = __ldg(body + i);
+        const float scale = __ldg(scales + (one_block ? 0 : (start + i * 16ll) / block));
+        int sum = __dp4a(static_cast<int>(w.x), static_cast<int>(w.x), 0);
+        sum = __dp4a(static_cast<int>(w.y), static_cast<int>(w.y), sum);
+        sum = __dp4a(static_cast<int>(w.z), static_cast<int>(w.z), sum);
+        sum = __dp4a(static_cast<int>(w.w), static_cast<int>(w.w), sum);
+        a += scale_square(scale) * static_cast<double>(sum);
+    }
+    for (int i = vectors * 16 + threadIdx.x; i < n; i += kThreads) {
+        const int code = payload[start + i];
+        const float scale = __ldg(scales + (one_block ? 0 : (start + i) / block));
+        a += scale_square(scale) * static_cast<double>(code * code);
+    }
+    return a;
+}
+
+__global__ void __launch_bounds__(kThreads)
+tensor_list_squares_kernel(const nntrain_gradient_tensor* __restrict__ tensors, const Chunk* __restrict__ chunks,
+                           int chunk_values, double* __restrict__ partials) {
+    let_next_start();
+    const Chunk chunk = chunks[blockIdx.x];
+    const nntrain_gradient_tensor t = tensors[chunk.tensor];
+    const long long start = static_cast<long long>(chunk.index) * chunk_values;
+    const long long left = t.length - start;
+    const int n = static_cast<int>(left < chunk_values ? left : chunk_values);
+    double squares;
+    if (t.kind == kKindF32) {
+        squares = chunk_squares_f32(static_cast<const float*>(t.values) + start, n);
+    } else if (t.kind == kKindBf16) {
+        squares = chunk_squares_bf16(static_cast<const unsigned short*>(t.values) + start, n);
+    } else {
+        const bool one_block = t.block_size == 0 || t.block_size >= t.length;
+        squares = chunk_squares_bfp8(static_cast<const signed char*>(t.values), t.scales, start, n,
+                                     t.block_size, one_block);
+    }
+    cta_store_partial(squares, partials);
+}
+
+// One CTA.  A warp sums the partials of a tensor (a lane takes every 32nd, then
+// a butterfly), lane 0 keeps the running total of the warp's tensors, the 32
+// totals are summed in warp order.
+__global__ void __launch_bounds__(kFinishThreads)
+tensor_list_finish_kernel(const nntrain_gradient_tensor* __restrict__ tensors, int count, long long chunks,
+                          const double* partials, float max_norm, float* norm_and_coefficient, float* tensor_norms,
+                          int* finite_status) {
+    __shared__ double totals[kFinishThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    wait_for_previous();
+    let_next_start();
+    double total = 0.0;
+    for (int t = warp; t < count; t += kFinishThreads / 32) {
+        const long long first = tensors[t].first_chunk, end = t + 1 < count ? tensors[t + 1].first_chunk : chunks;
+        double sums[8] = {};
+        long long i = first + lane;
+        for (; i + 7 * 32 < end; i += 8 * 32) {
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) sums[j] += partials[i + j * 32];
+        }
+        for (; i < end; i += 32) sums[0] += partials[i];
+        const double squares = warp_sum(((sums[0] + sums[1]) + (sums[2] + sums[3])) + ((sums[4] + sums[5]) + (sums[6] + sums[7])));
+        if (tensor_norms != nullptr && lane == 0) tensor_norms[t] = static_cast<float>(sqrt(squares));
+        total += squares;
+    }
+    if (lane == 0) totals[warp] = total;
+    __syncthreads();
+    if (warp == 0) {
+        const double squares = warp_sum(totals[lane]);
+        if (lane == 0) {
+            const float norm = static_cast<float>(sqrt(squares));
+            float c = 1.0f;
+            if (is_non_finite(norm)) {
+                if (finite_status != nullptr) *finite_status = 1;
+            } else if (norm > max_norm) {
+                c = __fdiv_rn(max_norm, __fadd_rn(norm, 1e-6f));
+            }
+            norm_and_coefficient[0] = norm;
+            norm_and_coefficient[1] = c;
+        }
+    }
+}
+
+// ---- clip ---------------------------------------------------------------------
+
+template <int kKind>
+__device__ __forceinline__ uint4 scaled(uint4 v, float c) {
+    if constexpr (kKind == kKindF32) {
+        return make_uint4(__float_as_uint(__fmul_rn(__uint_as_float(v.x), c)), __float_as_uint(__fmul_rn(__uint_as_float(v.y), c)),
+                          __float_as_uint(__fmul_rn(__uint_as_float(v.z), c)), __float_as_uint(__fmul_rn(__uint_as_float(v.w), c)));
+    } else {
+        return make_uint4(pack_bf16(__fmul_rn(bf16_low(v.x), c), __fmul_rn(bf16_high(v.x), c)),
+                          pack_bf16(__fmul_rn(bf16_low(v.y), c), __fmul_rn(bf16_high(v.y), c)),
+                          pack_bf16(__fmul_rn(bf16_low(v.z), c), __fmul_rn(bf16_high(v.z), c)),
+                          pack_bf16(__fmul_rn(bf16_low(v.w), c), __fmul_rn(bf16_high(v.w), c)));
+    }
+}
+
+// The 16 bytes that start `shift` bytes into the 32 bytes a, b.
+__device__ __forceinline__ uint4 shifted(uint4 a, uint4 b, int shift) {
+    const int words = shift >> 2, bits = (shift & 3) * 8;
+    unsigned w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (words & 2) {
+        #pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (words & 1) {
+        #pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                      __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
+// destination[start, start + n) = source[start, start + n) * c; c == 1 copies
+// the bits.  Stores are whole 16-byte words of the destination.  Where the
+// source lies differently to the 16-byte grid (a leaf gathered to its
+// running-sum offset in an arena), a word is put together from the two source
+// words around it; the second is the neighbouring thread's first, so it comes
+// from L1.  Words next to the ends of the tensor, whose source words would
+// reach outside of it, go value by value.
+template <int kKind, typename T>
+__device__ void clip_chunk(const T* source, T* destination, long long length, long long start, int n, float c) {
+    constexpr int kBytes = sizeof(T), kPerWord = 16 / kBytes;
+    const T* from = source + start;
+    T* to = destination + start;
+    const int head = head_values(to, kBytes, n), words = (n - head) / kPerWord, tail = head + words * kPerWord;
+    const bool copy = c == 1.0f;
+    auto one = [&](int i) {
+        if (copy) {
+            to[i] = from[i];
+        } else if constexpr (kKind == kKindF32) {
+            to[i] = __fmul_rn(from[i], c);
+        } else {
+            to[i] = bf16_bits(__fmul_rn(bf16_value(from[i]), c));
+        }
+    };
+    if (static_cast<int>(threadIdx.x) < head) one(threadIdx.x);
+    if (tail + static_cast<int>(threadIdx.x) < n) one(tail + threadIdx.x);
+    uint4* out = reinterpret_cast<uint4*>(to + head);
+    const int shift = static_cast<int>(reinterpret_cast<std::uintptr_t>(from + head) & 15u);
+    if (shift == 0) {
+        const uint4* in = reinterpret_cast<const uint4*>(from + head);
+        for (int i = threadIdx.x; i < words; i += kUnroll * kThreads) {
+            uint4 v[kUnroll];
+            #pragma unroll
+            for (int j = 0; j < kUnroll; ++j)
+                if (i + j * kThreads < words) v[j] = __ldcs(in + i + j * kThreads);
+            #pragma unroll
+            for (int j = 0; j < kUnroll; ++j)
+                if (i + j * kThreads < words) __stcs(out + i + j * kThreads, copy ? v[j] : scaled<kKind>(v[j], c));
+        }
+        return;
+    }
+    const uint4* in = reinterpret_cast<const uint4*>(reinterpret_cast<std::uintptr_t>(from + head) - shift);
+    const uint4* first = reinterpret_cast<const uint4*>(source);
+    const uint4* last = reinterpret_cast<const uint4*>(source + length);
+    auto inside = [&](int i) {
+        return reinterpret_cast<std::uintptr_t>(in + i) >= reinterpret_cast<std::uintptr_t>(first) &&
+               reinterpret_cast<std::uintptr_t>(in + i + 2) <= reinterpret_cast<std::uintptr_t>(last);
+    };
+    for (int i = threadIdx.x; i < words; i += kUnroll * kThreads) {
+        uint4 a[kUnroll], b[kUnroll];
+        #pragma unroll
+        for (int j = 0; j < kUnroll; ++j) {
+            const int w = i + j * kThreads;
+            if (w < words && inside(w)) {
+                a[j] = __ldg(in + w);
+                b[j] = __ldg(in + w + 1);
+            }
+        }
+        #pragma unroll
+        for (int j = 0; j < kUnroll; ++j) {
+            const int w = i + j * kThreads;
+            if (w >= words) continue;
+            if (inside(w)) {
+                const uint4 v = shifted(a[j], b[j], shift);
+                __stcs(out + w, copy ? v : scaled<kKind>(v, c));
+            } else {
+                for (int k = 0; k < kPerWord; ++k) one(head + w * kPerWord + k);
+            }
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kThreads)
+tensor_list_clip_kernel(const nntrain_gradient_tensor* __restrict__ tensors, const Chunk* __restrict__ chunks,
+                        int chunk_values, const float* norm_and_coefficient) {
+    // from the back: what the squares pass read last is read first
+    const Chunk chunk = chunks[gridDim.x - 1 - blockIdx.x];
+    const nntrain_gradient_tensor t = tensors[chunk.tensor];
+    const long long start = static_cast<long long>(chunk.index) * chunk_values;
+    const long long left = t.length - start;
+    const int n = static_cast<int>(left < chunk_values ? left : chunk_values);
+    wait_for_previous();
+    const float c = norm_and_coefficient[1];
+    if (t.kind == kKindBfp8) {
+        // scale' = max(scale * c, FLT_MIN), payload untouched: the blocks whose
+        // first value is in this chunk
+        float* out = t.destination != nullptr ? static_cast<float*>(t.destination) : t.scales;
+        if (c == 1.0f && out == t.scales) return;
+        const long long block = t.block_size == 0 || t.block_size >= t.length ? t.length : t.block_size;
+        const long long first = (start + block - 1) / block, end = (start + n - 1) / block + 1;
+        for (long long b = first + threadIdx.x; b < end; b += kThreads)
+            out[b] = c == 1.0f ? t.scales[b] : fmaxf(__fmul_rn(t.scales[b], c), FLT_MIN);
+        return;
+    }
+    void* out = t.destination != nullptr ? t.destination : const_cast<void*>(t.values);
+    if (c == 1.0f && out == t.values) return;
+    if (t.kind == kKindF32)
+        clip_chunk<kKindF32>(static_cast<const float*>(t.values), static_cast<float*>(out), t.length, start, n, c);
+    else
+        clip_chunk<kKindBf16>(static_cast<const unsigned short*>(t.values), static_cast<unsigned short*>(out), t.length, start, n, c);
+}
+
+bool valid_tensor(const nntrain_gradient_tensor& t) {
+    if (t.length < 0 || t.block_size < 0 || t.kind < kKindF32 || t.kind > kKindBfp8) return false;
+    if (t.length == 0) return true;
+    if (t.values == nullptr || (t.kind == kKindBfp8 && t.scales == nullptr)) return false;
+    const std::uintptr_t bytes = t.kind == kKindF32 ? 4 : (t.kind == kKindBf16 ? 2 : 1);
+    return aligned_for(t.values, bytes) && aligned_for(t.scales, 4) &&
+           aligned_for(t.destination, t.kind == kKindBfp8 ? 4 : bytes);
+}
+
+int plan_list(nntrain_gradient_tensor* tensors, int count, int* chunk_map, long long capacity,
+              long long* chunk_count, int* chunk_values) {
+    if (!tensors || count <= 0 || !chunk_count || !chunk_values || capacity < 0)
+        return static_cast<int>(cudaErrorInvalidValue);
+    long long total = 0;
+    for (int i = 0; i < count; ++i) {
+        if (!valid_tensor(tensors[i]) || tensors[i].length > (1ll << 46) - total) return static_cast<int>(cudaErrorInvalidValue);
+        total += tensors[i].length;
+    }
+    long long size = (total / 65536 + kChunkLeast - 1) / kChunkLeast * kChunkLeast;
+    size = size < kChunkLeast ? kChunkLeast : (size > kChunkMost ? kChunkMost : size);
+    long long chunks = 0;
+    for (int i = 0; i < count; ++i) {
+        tensors[i].first_chunk = chunks;
+        const long long here = (tensors[i].length + size - 1) / size;
+        if (chunk_map != nullptr) {
+            if (chunks + here > capacity) return static_cast<int>(cudaErrorInvalidValue);
+            for (long long k = 0; k < here; ++k) {
+                chunk_map[2 * (chunks + k)] = i;
+                chunk_map[2 * (chunks + k) + 1] = static_cast<int>(k);
+            }
+        }
+        chunks += here;
+    }
+    if (chunks > 2147483647ll) return static_cast<int>(cudaErrorInvalidValue);
+    *chunk_count = chunks;
+    *chunk_values = static_cast<int>(size);
+    return static_cast<int>(cudaSuccess);
+}
+
+int clip_list(int device, const nntrain_gradient_tensor* tensors, int count, const int* chunk_map,
+              long long chunk_count, int chunk_values, double* workspace, float max_norm, int apply,
+              float* norm_and_coefficient, float* tensor_norms, int* finite_status, cudaStream_t stream) {
+    if (!tensors || count <= 0 || chunk_count < 0 || chunk_count > 2147483647ll || chunk_values < kChunkLeast ||
+        chunk_values > kChunkMost || chunk_values % kChunkLeast != 0 || !norm_and_coefficient || !(max_norm > 0.0f) ||
+        (chunk_count > 0 && (!chunk_map || !workspace)) || !aligned_for(chunk_map, 8) || !aligned_for(workspace, 8))
+        return static_cast<int>(cudaErrorInvalidValue);
+    const DeviceScope scope(device);
+    if (scope.status() != cudaSuccess) return scope.status();
+    const Chunk* chunks = reinterpret_cast<const Chunk*>(chunk_map);
+    const int grid = static_cast<int>(chunk_count);
+    cudaError_t e = cudaSuccess;
+    if (grid > 0) {
+        tensor_list_squares_kernel<<<grid, kThreads, 0, stream>>>(tensors, chunks, chunk_values, workspace);
+        e = cudaPeekAtLastError();
+    }
+    if (e == cudaSuccess)
+        e = launch_dependent(tensor_list_finish_kernel, 1, kFinishThreads, 0, stream, tensors, count, chunk_count,
+                             workspace, max_norm, norm_and_coefficient, tensor_norms, finite_status);
+    if (e == cudaSuccess && apply && grid > 0)
+        e = launch_dependent(tensor_list_clip_kernel, grid, kThreads, 0, stream, tensors, chunks, chunk_values,
+                             norm_and_coefficient);
+    return static_cast<int>(e);
+}
+
+}  // namespace
+}  // namespace ngb
+
+using namespace ngb;
+
+NNTRAIN_EXPORT int nntrain_gradient_list_plan(nntrain_gradient_tensor* tensors, int count, int* chunk_map,
+                                              long long capacity, long long* chunk_count, int* chunk_values) {
+    return complete(kOpTensorList, -1, plan_list(tensors, count, chunk_map, capacity, chunk_count, chunk_values));
+}
+
+NNTRAIN_EXPORT int nntrain_gradient_list_clip(int device, const nntrain_gradient_tensor* tensors, int count,
+                                              const int* chunk_map, long long chunk_count, int chunk_values,
+                                              double* workspace, float max_norm, int apply,
+                                              float* norm_and_coefficient, float* tensor_norms, int* finite_status,
+                                              nntrain_stream_t stream) {
+    return complete(kOpTensorList, device,
+                    clip_list(device, tensors, count, chunk_map, chunk_count, chunk_values, workspace, max_norm, apply,
+                              norm_and_coefficient, tensor_norms, finite_status, static_cast<cudaStream_t>(stream)));
+}

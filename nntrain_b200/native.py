@@ -9,9 +9,14 @@ buffers.
   CudaGradientBuckets     NNtrain.Core/Tensors/CudaGradientBuckets.cs:6-349
   GradientNorm            the norm / clip kernels behind
                           NNtrain.Core/Tensors/Tensor.CudaKernels.cs:119-854
+  GradientTensorList      the leaves that clip_grad_norm_ walks there, as one
+                          table (NNtrain.Core/Torch/nn.cs:32-81)
 """
 from __future__ import annotations
 
+import ctypes
+
+import numpy as np
 import torch
 
 from .library import check, load
@@ -38,6 +43,35 @@ def _require(t: torch.Tensor, dtype, name: str, device: int | None = None) -> No
         raise ValueError(f"{name} must be contiguous")
     if device is not None and t.device.index != device:
         raise ValueError(f"{name} is on device {t.device.index}, expected {device}")
+
+
+_FLOAT32, _BFLOAT16 = (torch.float32,), (torch.bfloat16, torch.int16)   # bf16 values, or their bits
+_FLOATS = _FLOAT32 + _BFLOAT16
+
+
+def _kind(t: torch.Tensor) -> int:
+    """0 = fp32, 1 = bf16 (the kinds of the C boundary)."""
+    return 0 if t.dtype == torch.float32 else 1
+
+
+def _stream_on(device: int, stream):
+    """(handle, context) of `stream`, or of the device's current stream.  Scratch
+    that a call allocates under the context belongs to that stream, so it is not
+    handed out again before the call's kernels have run."""
+    if stream is None:
+        return torch.cuda.current_stream(device).cuda_stream, torch.cuda.device(device)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    return stream.cuda_stream, torch.cuda.stream(stream)
+
+
+def _scratch(device: int, bytes_: int, stream):
+    """(stream handle, scratch tensor or None) for one call."""
+    handle, context = _stream_on(device, stream)
+    if bytes_ == 0:
+        return handle, None
+    with context:
+        return handle, torch.empty(bytes_, dtype=torch.uint8, device=f"cuda:{device}")
 
 
 def scale_count(length: int, block_size: int) -> int:
@@ -324,6 +358,61 @@ class CudaGradientBuckets:
         check("gradient_comm_destroy", load().nntrain_gradient_comm_destroy(device, stream))
 
 
+class GradientTensorList:
+    """The gradient tensors of a model as one table on the device: fp32, bf16 and
+    BFP8 (payload, with its scales and block size) tensors of any length and
+    place, each with an optional destination for its clipped values (BFP8: its
+    clipped scales); without one it is clipped in place.  Build it once for
+    leaves that stay where they are; it holds on to the tensors."""
+
+    _TENSOR = np.dtype([("values", np.uint64), ("scales", np.uint64), ("destination", np.uint64),
+                        ("length", np.int64), ("first_chunk", np.int64), ("kind", np.int32), ("block_size", np.int32)])
+
+    def __init__(self, device: int, tensors, scales=None, block_sizes=None, destinations=None):
+        count = len(tensors)
+        scales = [None] * count if scales is None else list(scales)
+        block_sizes = [0] * count if block_sizes is None else list(block_sizes)
+        destinations = [None] * count if destinations is None else list(destinations)
+        if count == 0 or not len(scales) == len(block_sizes) == len(destinations) == count:
+            raise ValueError("a gradient list needs tensors, and one scale, block size and destination for each of them")
+        table = np.zeros(count, dtype=self._TENSOR)
+        for i, (t, s, block, to) in enumerate(zip(tensors, scales, block_sizes, destinations)):
+            if t.dtype not in _FLOATS + (torch.int8,):
+                raise ValueError(f"tensor {i} must be float32, bfloat16 or an int8 payload, got {t.dtype}")
+            _require(t, t.dtype, f"tensor {i}", device)
+            encoded = t.dtype == torch.int8
+            if encoded:
+                if s is None or block < 0:
+                    raise ValueError(f"tensor {i} is a BFP8 payload: it needs its scales and block size")
+                _require(s, torch.float32, f"scales of tensor {i}", device)
+                if t.numel() and s.numel() != scale_count(t.numel(), block):
+                    raise ValueError(f"tensor {i}: payload / scale lengths do not match the descriptor")
+            elif s is not None:
+                raise ValueError(f"tensor {i} is not a BFP8 payload: it has no scales")
+            if to is not None:
+                _require(to, torch.float32 if encoded else to.dtype, f"destination of tensor {i}", device)
+                source = s if encoded else t
+                if not encoded and (to.dtype not in _FLOATS or _kind(to) != _kind(t)):
+                    raise ValueError(f"destination of tensor {i} must have its type")
+                if to.numel() != source.numel():
+                    raise ValueError(f"destination of tensor {i} must have its length")
+                apart = abs(to.data_ptr() - source.data_ptr())
+                if 0 < apart < source.numel() * source.element_size():
+                    raise ValueError(f"destination of tensor {i} overlaps it")
+            table[i] = (t.data_ptr(), _ptr(s) if encoded else 0, _ptr(to), t.numel(), 0,
+                        2 if encoded else _kind(t), block if encoded else 0)
+        chunks, values = ctypes.c_longlong(), ctypes.c_int()
+        plan = load().nntrain_gradient_list_plan
+        check("gradient_list_plan", plan(table.ctypes.data, count, None, 0, ctypes.addressof(chunks), ctypes.addressof(values)))
+        chunk_map = np.zeros((max(chunks.value, 1), 2), dtype=np.int32)
+        check("gradient_list_plan", plan(table.ctypes.data, count, chunk_map.ctypes.data, chunks.value,
+                                         ctypes.addressof(chunks), ctypes.addressof(values)))
+        self.device, self.count, self.chunks, self.chunk_values = device, count, chunks.value, values.value
+        self.table = torch.from_numpy(table.view(np.uint8)).to(f"cuda:{device}")
+        self.chunk_map = torch.from_numpy(chunk_map).to(f"cuda:{device}")
+        self._held = (list(tensors), scales, destinations)
+
+
 class GradientNorm:
     """Sum of squares and clip kernels (kinds: 0 fp32, 1 bf16, 2 BFP8)."""
 
@@ -346,6 +435,38 @@ class GradientNorm:
     def clip_apply(device: int, kind: int, values, multiplier: float = 1.0, coefficient=None, stream=None) -> None:
         check("gradient_clip_apply", load().nntrain_gradient_clip_apply(
             device, kind, _ptr(values), values.numel(), multiplier, _ptr(coefficient), _stream(stream)))
+
+    @staticmethod
+    def clip_tensors(device: int, tensors: GradientTensorList, max_norm: float, norm_and_coefficient,
+                     tensor_norms=None, finite_status=None, apply: bool = True, workspace=None, stream=None) -> None:
+        """The global norm over a list and, with `apply`, the clip of every tensor
+        of it, in three launches and without a host read.  `workspace` (optional):
+        at least `tensors.chunks` float64 values that no call in flight at the
+        same time uses."""
+        if tensors.device != device:
+            raise ValueError(f"the list is on device {tensors.device}, expected {device}")
+        _require(norm_and_coefficient, torch.float32, "norm_and_coefficient", device)
+        if norm_and_coefficient.numel() < 2:
+            raise ValueError("norm_and_coefficient needs two values")
+        if not max_norm > 0.0:
+            raise ValueError("max_norm must be positive")
+        if tensor_norms is not None:
+            _require(tensor_norms, torch.float32, "tensor_norms", device)
+            if tensor_norms.numel() < tensors.count:
+                raise ValueError("tensor_norms needs one value for each tensor")
+        if finite_status is not None:
+            _require(finite_status, torch.int32, "finite_status", device)
+        if workspace is None:
+            handle, workspace = _scratch(device, tensors.chunks * 8, stream)
+        else:
+            _require(workspace, torch.float64, "workspace", device)
+            if workspace.numel() < tensors.chunks:
+                raise ValueError("workspace is too small")
+            handle = _stream_on(device, stream)[0]
+        check("gradient_list_clip", load().nntrain_gradient_list_clip(
+            device, tensors.table.data_ptr(), tensors.count, tensors.chunk_map.data_ptr(), tensors.chunks,
+            tensors.chunk_values, _ptr(workspace), max_norm, int(apply), norm_and_coefficient.data_ptr(),
+            _ptr(tensor_norms), _ptr(finite_status), handle))
 
 
 class Bfp8GradientOptimizers:

@@ -1,0 +1,101 @@
+"""The chunk plan of a gradient list and the refusals of its entry points: host
+code, no device needed."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from nntrain_b200.native import GradientTensorList
+
+INVALID = 1   # cudaErrorInvalidValue
+TENSOR = GradientTensorList._TENSOR
+
+
+def table_of(lengths, kind=0, block=0):
+    table = np.zeros(len(lengths), dtype=TENSOR)
+    table["values"], table["length"], table["kind"], table["block_size"] = 4096, lengths, kind, block
+    if kind == 2:
+        table["scales"] = 4096
+    return table
+
+
+def plan(lib, table, chunk_map=None, capacity=None):
+    chunks, values = ctypes.c_longlong(), ctypes.c_int()
+    status = lib.nntrain_gradient_list_plan(
+        table.ctypes.data, len(table), None if chunk_map is None else chunk_map.ctypes.data,
+        (0 if chunk_map is None else len(chunk_map)) if capacity is None else capacity,
+        ctypes.addressof(chunks), ctypes.addressof(values))
+    return status, chunks.value, values.value
+
+
+@pytest.mark.parametrize("lengths", (
+    [1], [0, 5, 0], [4096, 4097, 1, 0, 8191, 8192], [233_373_696] + [1536, 256, 2_359_296] * 28, [1] * 400, [3_000_000_000]))
+def test_plan_covers_every_value_once(lib, lengths):
+    table = table_of(lengths)
+    status, chunks, size = plan(lib, table)
+    assert status == 0 and 4096 <= size <= 65536 and size % 4096 == 0
+    chunk_map = np.full((max(chunks, 1), 2), -1, dtype=np.int32)
+    status, again, size_again = plan(lib, table, chunk_map, chunks)
+    assert status == 0 and (again, size_again) == (chunks, size)
+    assert chunks == sum(-(-n // size) for n in lengths)
+    first = np.concatenate([[0], np.cumsum([-(-n // size) for n in lengths])])
+    assert (table["first_chunk"] == first[:-1]).all()
+    for t, n in enumerate(lengths):
+        mine = chunk_map[first[t]:first[t + 1]]
+        assert (mine[:, 0] == t).all() and (mine[:, 1] == np.arange(len(mine))).all()
+        assert (len(mine) - 1) * size < n <= len(mine) * size if n else len(mine) == 0
+
+
+def test_plan_bounds_the_partials_of_one_finish_block(lib):
+    status, chunks, _ = plan(lib, table_of([1_543_714_304]))
+    assert status == 0 and chunks <= 65536
+
+
+def test_plan_refusals(lib):
+    chunks, values = ctypes.c_longlong(), ctypes.c_int()
+    a, b = ctypes.addressof(chunks), ctypes.addressof(values)
+    good = table_of([10])
+    assert lib.nntrain_gradient_list_plan(None, 1, None, 0, a, b) == INVALID
+    assert lib.nntrain_gradient_list_plan(good.ctypes.data, 0, None, 0, a, b) == INVALID
+    assert lib.nntrain_gradient_list_plan(good.ctypes.data, 1, None, 0, None, b) == INVALID
+    assert lib.nntrain_gradient_list_plan(good.ctypes.data, 1, None, -1, a, b) == INVALID
+    for field, value in (("length", -1), ("kind", 3), ("kind", -1), ("block_size", -1), ("values", 0),
+                         ("values", 4098), ("destination", 4097)):
+        bad = table_of([10])
+        bad[field] = value
+        assert plan(lib, bad)[0] == INVALID, (field, value)
+    unscaled = table_of([10], kind=2, block=32)
+    unscaled["scales"] = 0
+    assert plan(lib, unscaled)[0] == INVALID
+    assert plan(lib, table_of([1 << 62, 1 << 62]))[0] == INVALID                # the sum of lengths would overflow
+    small = np.zeros((1, 2), dtype=np.int32)
+    assert plan(lib, table_of([10_000]), small, 1)[0] == INVALID                # room for one chunk of three
+
+
+def test_clip_refusals_come_before_the_device(lib):
+    def call(tensors=4096, count=1, chunk_map=4096, chunks=1, values=4096, workspace=4096, max_norm=1.0, out=4096):
+        return lib.nntrain_gradient_list_clip(0, tensors, count, chunk_map, chunks, values, workspace, max_norm, 1, out,
+                                              None, None, None)
+    assert call(tensors=None) == INVALID
+    assert call(count=0) == INVALID
+    assert call(chunk_map=None) == INVALID
+    assert call(chunk_map=4100) == INVALID
+    assert call(chunks=-1) == INVALID
+    assert call(chunks=1 << 31) == INVALID
+    assert call(values=4095) == INVALID
+    assert call(values=1 << 20) == INVALID
+    assert call(workspace=None) == INVALID
+    assert call(workspace=4100) == INVALID
+    assert call(out=None) == INVALID
+    for max_norm in (0.0, -1.0, float("nan")):
+        assert call(max_norm=max_norm) == INVALID
+
+
+def test_a_list_refuses_tensors_that_are_not_on_a_device():
+    import torch
+    with pytest.raises(ValueError, match="CUDA"):
+        GradientTensorList(0, [torch.zeros(4)])
+    with pytest.raises(ValueError, match="needs tensors"):
+        GradientTensorList(0, [])
+    with pytest.raises(ValueError, match="float32, bfloat16 or an int8"):
+        GradientTensorList(0, [torch.zeros(4, dtype=torch.float16)])
