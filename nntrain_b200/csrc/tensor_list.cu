@@ -4,10 +4,12 @@
 // The reference walks the leaves: one sum-of-squares launch and one scale
 // launch per tensor with a host read between them (NNtrain.Core/Tensors/
 // Tensor.CudaKernels.cs:119-854, NNtrain.Core/Torch/nn.cs:32-81).  Here a table
-// of the tensors lies on the device and three launches serve all of them:
+// of the tensors lies on the device and two or three launches serve all of
+// them:
 //
 //   squares   one CTA per chunk of a tensor -> one binary64 partial per chunk
-//   finish    one CTA: partials -> tensor norms -> norm and coefficient
+//   finish    partials -> tensor norms, norm and coefficient (short lists: in
+//             the clip)
 //   clip      one CTA per chunk again: destination = value * coefficient
 //
 //   n_t = sqrt(sum of v^2),  n = (float)sqrt(sum of n_t^2),
@@ -35,15 +37,26 @@ enum TensorKind : int { kKindF32 = 0, kKindBf16 = 1, kKindBfp8 = 2 };
 constexpr int kUnroll = 4;              // 128-bit loads in flight per thread
 constexpr int kFinishThreads = 1024;
 
-// A chunk is 4096 values at least (one trip of a CTA over fp32) and grows with
-// the list so that the finish kernel, one CTA, has at most about 64 Ki
-// partials; 65536 at most, so that the last wave of CTAs stays short.
-constexpr long long kChunkLeast = 4096, kChunkMost = 65536;
+// A chunk is the same number of bytes for every kind: chunk_values fp32 values,
+// twice as many bf16 and four times as many BFP8 ones.  It grows with the list
+// (a 2048th of it) from 16 KB, one trip of a CTA, where a short list still
+// covers the SMs, to 96 KB.  Measured on the 41.6 M-value bf16 list: 52 us with
+// 16 KB chunks, 45 us with 48 KB, 47 us with 96 KB; on 1.54 G fp32 values 2.68 ms
+// with 96 KB and 2.71 ms with 256 KB.
+constexpr long long kChunkLeast = 4096, kChunkMost = 24576;
+
+// Lists of at most this many chunks are finished by every CTA of the clip on
+// its own, which saves a launch and its latency.
+constexpr long long kFusedFinishChunks = 1024;
 
 struct alignas(8) Chunk {
     int tensor;
-    unsigned index;                     // values [index, index + 1) * chunk_values of the tensor
+    unsigned index;                     // the tensor's values [index, index + 1) * kind_values()
 };
+
+__host__ __device__ __forceinline__ long long kind_values(int chunk_values, int kind) {
+    return static_cast<long long>(chunk_values) << kind;
+}
 
 __device__ __forceinline__ double square_of(float v) {
     const double d = static_cast<double>(v);
@@ -151,9 +164,8 @@ tensor_list_squares_kernel(const nntrain_gradient_tensor* __restrict__ tensors, 
     let_next_start();
     const Chunk chunk = chunks[blockIdx.x];
     const nntrain_gradient_tensor t = tensors[chunk.tensor];
-    const long long start = static_cast<long long>(chunk.index) * chunk_values;
-    const long long left = t.length - start;
-    const int n = static_cast<int>(left < chunk_values ? left : chunk_values);
+    const long long values = kind_values(chunk_values, t.kind), start = chunk.index * values;
+    const int n = static_cast<int>(t.length - start < values ? t.length - start : values);
     double squares;
     if (t.kind == kKindF32) {
         squares = chunk_squares_f32(static_cast<const float*>(t.values) + start, n);
@@ -167,47 +179,81 @@ tensor_list_squares_kernel(const nntrain_gradient_tensor* __restrict__ tensors, 
     cta_store_partial(squares, partials);
 }
 
-// One CTA.  A warp sums the partials of a tensor (a lane takes every 32nd, then
-// a butterfly), lane 0 keeps the running total of the warp's tensors, the 32
-// totals are summed in warp order.
+// Sum of values[first, end): thread `at` of `step` takes every step-th one.
+__device__ __forceinline__ double strided_sum(const double* values, long long first, long long end, int at, int step) {
+    double sums[4] = {};
+    long long i = first + at;
+    for (; i + 3 * step < end; i += 4 * step) {
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) sums[j] += values[i + j * step];
+    }
+    for (; i < end; i += step) sums[0] += values[i];
+    return (sums[0] + sums[1]) + (sums[2] + sums[3]);
+}
+
+constexpr int kSumLanes = 1024;         // lanes of the fixed summation order, whatever the CTA's size
+
+// The sum of all partials, the same bits for every CTA size: virtual lane v of
+// 1024 takes every 1024th, the lanes are summed by warps, the warps in order.
+// To be called by all threads of a CTA of kCtaThreads; the result is valid in
+// its first warp.
+template <int kCtaThreads>
+__device__ double sum_of_partials(const double* partials, long long chunks, double (&totals)[kSumLanes / 32]) {
+    const int lane = threadIdx.x & 31;
+    #pragma unroll
+    for (int v = threadIdx.x; v < kSumLanes; v += kCtaThreads) {
+        const double sum = warp_sum(strided_sum(partials, 0, chunks, v, kSumLanes));
+        if (lane == 0) totals[v >> 5] = sum;
+    }
+    __syncthreads();
+    return threadIdx.x < 32 ? warp_sum(totals[lane]) : 0.0;
+}
+
+struct NormResult { float norm, coefficient; };
+
+__device__ __forceinline__ NormResult norm_result(double squares, float max_norm) {
+    const float norm = static_cast<float>(sqrt(squares));
+    const bool clip = !is_non_finite(norm) && norm > max_norm;
+    return {norm, clip ? __fdiv_rn(max_norm, __fadd_rn(norm, 1e-6f)) : 1.0f};
+}
+
+__device__ __forceinline__ void store_result(NormResult r, float* norm_and_coefficient, int* finite_status) {
+    norm_and_coefficient[0] = r.norm;
+    norm_and_coefficient[1] = r.coefficient;
+    if (finite_status != nullptr && is_non_finite(r.norm)) *finite_status = 1;
+}
+
+// The norm of tensor t by one warp; t may be beyond the list.
+__device__ void store_tensor_norm(const nntrain_gradient_tensor* tensors, int count, long long chunks, int t,
+                                  const double* partials, float* tensor_norms) {
+    long long first = 0, end = 0;
+    if (t < count) {
+        first = tensors[t].first_chunk;
+        end = t + 1 < count ? tensors[t + 1].first_chunk : chunks;
+    }
+    wait_for_previous();
+    let_next_start();
+    const int lane = threadIdx.x & 31;
+    const double squares = warp_sum(strided_sum(partials, first, end, lane, 32));
+    if (t < count && lane == 0) tensor_norms[t] = static_cast<float>(sqrt(squares));
+}
+
+// CTA 0 sums all partials and leaves norm and coefficient; the others, there
+// when tensor_norms is asked for, take a tensor per warp.
 __global__ void __launch_bounds__(kFinishThreads)
 tensor_list_finish_kernel(const nntrain_gradient_tensor* __restrict__ tensors, int count, long long chunks,
                           const double* partials, float max_norm, float* norm_and_coefficient, float* tensor_norms,
                           int* finite_status) {
-    __shared__ double totals[kFinishThreads / 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ double totals[kSumLanes / 32];
+    if (blockIdx.x > 0) {
+        const int t = (blockIdx.x - 1) * (kFinishThreads / 32) + (threadIdx.x >> 5);
+        store_tensor_norm(tensors, count, chunks, t, partials, tensor_norms);
+        return;
+    }
     wait_for_previous();
     let_next_start();
-    double total = 0.0;
-    for (int t = warp; t < count; t += kFinishThreads / 32) {
-        const long long first = tensors[t].first_chunk, end = t + 1 < count ? tensors[t + 1].first_chunk : chunks;
-        double sums[8] = {};
-        long long i = first + lane;
-        for (; i + 7 * 32 < end; i += 8 * 32) {
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) sums[j] += partials[i + j * 32];
-        }
-        for (; i < end; i += 32) sums[0] += partials[i];
-        const double squares = warp_sum(((sums[0] + sums[1]) + (sums[2] + sums[3])) + ((sums[4] + sums[5]) + (sums[6] + sums[7])));
-        if (tensor_norms != nullptr && lane == 0) tensor_norms[t] = static_cast<float>(sqrt(squares));
-        total += squares;
-    }
-    if (lane == 0) totals[warp] = total;
-    __syncthreads();
-    if (warp == 0) {
-        const double squares = warp_sum(totals[lane]);
-        if (lane == 0) {
-            const float norm = static_cast<float>(sqrt(squares));
-            float c = 1.0f;
-            if (is_non_finite(norm)) {
-                if (finite_status != nullptr) *finite_status = 1;
-            } else if (norm > max_norm) {
-                c = __fdiv_rn(max_norm, __fadd_rn(norm, 1e-6f));
-            }
-            norm_and_coefficient[0] = norm;
-            norm_and_coefficient[1] = c;
-        }
-    }
+    const double squares = sum_of_partials<kFinishThreads>(partials, chunks, totals);
+    if (threadIdx.x == 0) store_result(norm_result(squares, max_norm), norm_and_coefficient, finite_status);
 }
 
 // ---- clip ---------------------------------------------------------------------
@@ -312,17 +358,49 @@ __device__ void clip_chunk(const T* source, T* destination, long long length, lo
     }
 }
 
+struct ClipArguments {
+    const nntrain_gradient_tensor* tensors;
+    const Chunk* chunks;
+    const double* partials;
+    float* norm_and_coefficient;
+    float* tensor_norms;
+    int* finite_status;
+    float max_norm;
+    int count, chunk_count, chunk_values;
+};
+
+// kFinish: norm and coefficient are not there yet; every CTA forms them from
+// the partials (the same bits in each), CTA 0 stores them, and CTAs behind the
+// chunks store the tensor norms.
+template <bool kFinish>
 __global__ void __launch_bounds__(kThreads)
-tensor_list_clip_kernel(const nntrain_gradient_tensor* __restrict__ tensors, const Chunk* __restrict__ chunks,
-                        int chunk_values, const float* norm_and_coefficient) {
+tensor_list_clip_kernel(ClipArguments a) {
+    if (kFinish && static_cast<int>(blockIdx.x) >= a.chunk_count) {
+        const int t = (blockIdx.x - a.chunk_count) * kWarpsPerCta + (threadIdx.x >> 5);
+        store_tensor_norm(a.tensors, a.count, a.chunk_count, t, a.partials, a.tensor_norms);
+        return;
+    }
     // from the back: what the squares pass read last is read first
-    const Chunk chunk = chunks[gridDim.x - 1 - blockIdx.x];
-    const nntrain_gradient_tensor t = tensors[chunk.tensor];
-    const long long start = static_cast<long long>(chunk.index) * chunk_values;
-    const long long left = t.length - start;
-    const int n = static_cast<int>(left < chunk_values ? left : chunk_values);
+    const Chunk chunk = a.chunks[a.chunk_count - 1 - blockIdx.x];
+    const nntrain_gradient_tensor t = a.tensors[chunk.tensor];
+    const long long values = kind_values(a.chunk_values, t.kind), start = chunk.index * values;
+    const int n = static_cast<int>(t.length - start < values ? t.length - start : values);
     wait_for_previous();
-    const float c = norm_and_coefficient[1];
+    float c;
+    if constexpr (kFinish) {
+        __shared__ double totals[kSumLanes / 32];
+        __shared__ float coefficient;
+        const double squares = sum_of_partials<kThreads>(a.partials, a.chunk_count, totals);
+        if (threadIdx.x == 0) {
+            const NormResult r = norm_result(squares, a.max_norm);
+            coefficient = r.coefficient;
+            if (blockIdx.x == 0) store_result(r, a.norm_and_coefficient, a.finite_status);
+        }
+        __syncthreads();
+        c = coefficient;
+    } else {
+        c = a.norm_and_coefficient[1];
+    }
     if (t.kind == kKindBfp8) {
         // scale' = max(scale * c, FLT_MIN), payload untouched: the blocks whose
         // first value is in this chunk
@@ -355,17 +433,18 @@ int plan_list(nntrain_gradient_tensor* tensors, int count, int* chunk_map, long 
               long long* chunk_count, int* chunk_values) {
     if (!tensors || count <= 0 || !chunk_count || !chunk_values || capacity < 0)
         return static_cast<int>(cudaErrorInvalidValue);
-    long long total = 0;
+    long long total = 0;                // in fp32 values
     for (int i = 0; i < count; ++i) {
         if (!valid_tensor(tensors[i]) || tensors[i].length > (1ll << 46) - total) return static_cast<int>(cudaErrorInvalidValue);
-        total += tensors[i].length;
+        total += tensors[i].length >> tensors[i].kind;
     }
-    long long size = (total / 65536 + kChunkLeast - 1) / kChunkLeast * kChunkLeast;
+    long long size = (total / 2048 + kChunkLeast - 1) / kChunkLeast * kChunkLeast;
     size = size < kChunkLeast ? kChunkLeast : (size > kChunkMost ? kChunkMost : size);
     long long chunks = 0;
     for (int i = 0; i < count; ++i) {
         tensors[i].first_chunk = chunks;
-        const long long here = (tensors[i].length + size - 1) / size;
+        const long long values = kind_values(static_cast<int>(size), tensors[i].kind);
+        const long long here = (tensors[i].length + values - 1) / values;
         if (chunk_map != nullptr) {
             if (chunks + here > capacity) return static_cast<int>(cudaErrorInvalidValue);
             for (long long k = 0; k < here; ++k) {
@@ -397,12 +476,19 @@ int clip_list(int device, const nntrain_gradient_tensor* tensors, int count, con
         tensor_list_squares_kernel<<<grid, kThreads, 0, stream>>>(tensors, chunks, chunk_values, workspace);
         e = cudaPeekAtLastError();
     }
-    if (e == cudaSuccess)
-        e = launch_dependent(tensor_list_finish_kernel, 1, kFinishThreads, 0, stream, tensors, count, chunk_count,
-                             workspace, max_norm, norm_and_coefficient, tensor_norms, finite_status);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    const ClipArguments a{tensors, chunks, workspace, norm_and_coefficient, tensor_norms, finite_status, max_norm, count,
+                          grid, chunk_values};
+    if (apply && grid > 0 && grid <= kFusedFinishChunks)
+        return static_cast<int>(launch_dependent(tensor_list_clip_kernel<true>,
+                                                 grid + (tensor_norms ? (count + kWarpsPerCta - 1) / kWarpsPerCta : 0),
+                                                 kThreads, 0, stream, a));
+    constexpr int kFinishWarps = kFinishThreads / 32;
+    e = launch_dependent(tensor_list_finish_kernel, 1 + (tensor_norms ? (count + kFinishWarps - 1) / kFinishWarps : 0),
+                         kFinishThreads, 0, stream, tensors, count, chunk_count, workspace, max_norm,
+                         norm_and_coefficient, tensor_norms, finite_status);
     if (e == cudaSuccess && apply && grid > 0)
-        e = launch_dependent(tensor_list_clip_kernel, grid, kThreads, 0, stream, tensors, chunks, chunk_values,
-                             norm_and_coefficient);
+        e = launch_dependent(tensor_list_clip_kernel<false>, grid, kThreads, 0, stream, a);
     return static_cast<int>(e);
 }
 

@@ -54,24 +54,24 @@ def _kind(t: torch.Tensor) -> int:
     return 0 if t.dtype == torch.float32 else 1
 
 
-def _stream_on(device: int, stream):
-    """(handle, context) of `stream`, or of the device's current stream.  Scratch
-    that a call allocates under the context belongs to that stream, so it is not
-    handed out again before the call's kernels have run."""
+def _stream_on(device: int, stream) -> int:
+    """The handle of `stream`, or of the device's current stream."""
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream, torch.cuda.device(device)
-    if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, device=device)
-    return stream.cuda_stream, torch.cuda.stream(stream)
+        return torch.cuda.current_stream(device).cuda_stream
+    return stream if isinstance(stream, int) else stream.cuda_stream
 
 
 def _scratch(device: int, bytes_: int, stream):
-    """(stream handle, scratch tensor or None) for one call."""
-    handle, context = _stream_on(device, stream)
+    """Device scratch for one call on `stream`.  It is allocated on that stream,
+    so it is not handed out again before the call's kernels have run."""
     if bytes_ == 0:
-        return handle, None
-    with context:
-        return handle, torch.empty(bytes_, dtype=torch.uint8, device=f"cuda:{device}")
+        return None
+    if stream is None:
+        return torch.empty(bytes_, dtype=torch.uint8, device=torch.device("cuda", device))
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(bytes_, dtype=torch.uint8, device=torch.device("cuda", device))
 
 
 def scale_count(length: int, block_size: int) -> int:
@@ -440,7 +440,7 @@ class GradientNorm:
     def clip_tensors(device: int, tensors: GradientTensorList, max_norm: float, norm_and_coefficient,
                      tensor_norms=None, finite_status=None, apply: bool = True, workspace=None, stream=None) -> None:
         """The global norm over a list and, with `apply`, the clip of every tensor
-        of it, in three launches and without a host read.  `workspace` (optional):
+        of it, without a host read.  `workspace` (optional):
         at least `tensors.chunks` float64 values that no call in flight at the
         same time uses."""
         if tensors.device != device:
@@ -457,16 +457,15 @@ class GradientNorm:
         if finite_status is not None:
             _require(finite_status, torch.int32, "finite_status", device)
         if workspace is None:
-            handle, workspace = _scratch(device, tensors.chunks * 8, stream)
+            workspace = _scratch(device, tensors.chunks * 8, stream)
         else:
             _require(workspace, torch.float64, "workspace", device)
             if workspace.numel() < tensors.chunks:
                 raise ValueError("workspace is too small")
-            handle = _stream_on(device, stream)[0]
         check("gradient_list_clip", load().nntrain_gradient_list_clip(
             device, tensors.table.data_ptr(), tensors.count, tensors.chunk_map.data_ptr(), tensors.chunks,
             tensors.chunk_values, _ptr(workspace), max_norm, int(apply), norm_and_coefficient.data_ptr(),
-            _ptr(tensor_norms), _ptr(finite_status), handle))
+            _ptr(tensor_norms), _ptr(finite_status), _stream_on(device, stream)))
 
 
 class Bfp8GradientOptimizers:

@@ -46,6 +46,13 @@ def test_plan_covers_every_value_once(lib, lengths):
         assert (len(mine) - 1) * size < n <= len(mine) * size if n else len(mine) == 0
 
 
+@pytest.mark.parametrize("kind", (0, 1, 2))
+def test_a_chunk_is_as_many_bytes_for_every_kind(lib, kind):
+    n = 100_000
+    status, chunks, size = plan(lib, table_of([n], kind=kind, block=32))
+    assert status == 0 and size == 4096 and chunks == -(-n // (size << kind))
+
+
 def test_plan_bounds_the_partials_of_one_finish_block(lib):
     status, chunks, _ = plan(lib, table_of([1_543_714_304]))
     assert status == 0 and chunks <= 65536
