@@ -168,7 +168,8 @@ cudaError_t launch_bfp8_decode(const signed char* payload, const float* scales, 
     if (!payload || !scales || !destination || length <= 0 || block <= 0) return cudaErrorInvalidValue;
     if (block > length) block = length;
     const long long words = (length + 3) / 4;
-    if (aligned_to(payload, 4) && aligned_to(destination, 16)) {
+    // a 4-value word must not straddle two blocks on the vector path
+    if (aligned_to(payload, 4) && aligned_to(destination, 16) && (block % 4 == 0 || block >= length)) {
         const int grid = codec_grid_for((words + kThreads * kDecodeUnroll - 1) / (kThreads * kDecodeUnroll), kCtasPerSm);
         if (block == 32) bfp8_decode_blocks_kernel<5><<<grid, kThreads, 0, stream>>>(payload, scales, destination, length, block);
         else if (block == 64) bfp8_decode_blocks_kernel<6><<<grid, kThreads, 0, stream>>>(payload, scales, destination, length, block);
