@@ -340,6 +340,43 @@ int nntrain_optimizer_adamw_bfp8_gradient(
     long long length, float beta1, float beta2, float learning_rate, float weight_decay,
     float update_scale, float scaled_epsilon, int apply_weight_decay, nntrain_stream_t stream);
 
+/* ---- root-mean-square norm (ABI minor 36; no counterpart in the reference's
+ * gradient path, whose 8-bit products encode their inputs with a launch of
+ * their own: NNtrain.Cuda/native/cuda_runtime_bridge.cu:1540-2118) ------------
+ * kind, y_kind, weight_kind, weight_gradient_kind: 0 = fp32, 1 = bf16.  Rows of
+ * inputs may lie any stride (in values, at least `width`) apart; outputs are
+ * contiguous.  Addresses need the alignment of their type only. */
+
+/* h = x + residual (residual optional), i = 1 / sqrt(mean(h^2) + epsilon),
+ * y = h * i * weight; fp32 arithmetic.  residual_out (optional, with a
+ * residual): h, may be x or residual itself when that is contiguous.
+ * inverse_rms (optional): i per row.  payload, scales (optional): y in the
+ * codec's flat layout, so block_size (0 = one scale a row) has to divide width;
+ * the codec's rules for values that are not finite hold.  y (at least one of y
+ * and payload): without a payload y itself, with one what the codes stand for.
+ * *finite_status (optional) = 1 when a mean square or a y is not finite. */
+int nntrain_rms_norm_forward(
+    int device, int kind, const void* x, long long x_stride, const void* residual,
+    long long residual_stride, const void* weight, int weight_kind, long long rows, int width,
+    float epsilon, void* residual_out, void* y, int y_kind, signed char* payload, float* scales,
+    int block_size, float* inverse_rms, int* finite_status, nntrain_stream_t stream);
+/* Host only: bytes of scratch that nntrain_rms_norm_backward needs. */
+int nntrain_rms_norm_backward_workspace(long long rows, int width, long long* bytes);
+/* The gradient of the above for y's gradient dy (the encode passes it through):
+ * with g = dy * weight and n = h * i, x_gradient = i * (g - n * mean(g * n))
+ * + residual_gradient, which is the gradient of x and of residual alike, and
+ * weight_gradient = sum over rows of dy * n, added to what is there when
+ * accumulate != 0.  residual_gradient (optional): the gradient that reaches h
+ * from elsewhere.  x_gradient may be y_gradient or residual_gradient itself
+ * when that is contiguous.  The scratch is the caller's, one for each call in
+ * flight.  Fixed summation order: same inputs, same bits. */
+int nntrain_rms_norm_backward(
+    int device, int kind, const void* y_gradient, long long y_stride, const void* residual_gradient,
+    long long residual_stride, const void* h, long long h_stride, const void* weight, int weight_kind,
+    const float* inverse_rms, long long rows, int width, void* x_gradient, void* weight_gradient,
+    int weight_gradient_kind, int accumulate, void* workspace, long long workspace_bytes,
+    nntrain_stream_t stream);
+
 /* ---- N-rank all-reduce, one process per GPU (ABI minor 36) -------------------
  * The reference's compressed reducers accept exactly two devices of one
  * process (NNtrain.Core/Training/CudaBfp8GradientAllReduce.cs:44-49,

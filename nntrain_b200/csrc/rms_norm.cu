@@ -1,0 +1,663 @@
+// Root-mean-square norm of x + residual with its output in the codec's 8 bits,
+// and its gradient (ABI minor 36).
+//
+//   h = x + residual,  i = 1 / sqrt(mean(h^2) + epsilon),  y = h * i * w
+//   scale = max|y| / 127 over a block (1 for a block of zeros),
+//   code  = clamp(rne(y / scale), +-127)
+//
+//   g = dy * w,  n = h * i,  dx = i * (g - n * mean(g * n)) + dh,  dw = sum over rows of dy * n
+//
+// The encode is the codec's (NNtrain.Core/Tensors/Bfp8Quantization.cs:188-274,
+// NNtrain.Cuda/native/cuda_runtime_bridge.cu:138-232) applied to y in
+// registers: y is not written in 16 or 32 bits to be read again by an encode
+// launch.  All arithmetic is fp32; h, y and dx are rounded once, when they are
+// stored.  The sum of squares uses the unrounded h.
+//
+// Layout: the threads of a CTA hold one row in registers, groups of 8
+// consecutive values (one 128-bit load of bf16, two of fp32) or single values
+// where the row does not lie on 16-byte boundaries (odd widths); the grid is
+// one resident wave and a CTA walks rows, so the weight is loaded once and the
+// weight's gradient stays in registers until the end.  Rows too long for
+// registers are read again for each pass (they are in L1 / L2 then).
+//
+// Bound: HBM.  bf16 with residual, block 32: 7.1 bytes a value forward
+// (x, residual, h, payload, scales), 8 backward.
+#include "bfp8_kernels.cuh"
+#include "operator_launch.cuh"
+
+#include "nntrain_grad_abi.h"
+
+#include <atomic>
+
+namespace ngb {
+namespace {
+
+constexpr int kRowThreads = 512;              // most threads on a row held in registers
+constexpr int kLoopThreads = 256;             // threads on a row that is not
+constexpr int kMostPartials = 1184;           // most CTAs that leave a partial weight gradient: 8 on each of 148 SMs
+constexpr int kJoinColumns = 32, kJoinRows = 32;
+
+struct RowSum {
+    float (*slots)[kRowThreads / 32];
+    int turn;
+};
+
+// Sum / maximum over the CTA, the same value in every thread.  Two sets of
+// slots take turns, so one barrier per reduction is enough: a set is written
+// again only behind the barrier of the other one.
+template <bool kMaximum>
+__device__ __forceinline__ float over_cta(float v, RowSum& s) {
+    #pragma unroll
+    for (int offset = 16; offset > 0; offset >>= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, v, offset);
+        v = kMaximum ? fmaxf(v, other) : __fadd_rn(v, other);
+    }
+    const int warps = blockDim.x >> 5;
+    if (warps == 1) return v;
+    float* slots = s.slots[s.turn];
+    s.turn ^= 1;
+    if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float total = slots[0];
+    for (int w = 1; w < warps; ++w) total = kMaximum ? fmaxf(total, slots[w]) : __fadd_rn(total, slots[w]);
+    return total;
+}
+
+// ---- loads and stores of a group -------------------------------------------------
+
+template <int kVec>
+__device__ __forceinline__ void load_group(const float* p, float (&v)[kVec]) {
+    if constexpr (kVec == 1) {
+        v[0] = *p;
+    } else {
+        const float4 a = load_f4(p), b = load_f4(p + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+}
+template <int kVec>
+__device__ __forceinline__ void load_group(const unsigned short* p, float (&v)[kVec]) {
+    if constexpr (kVec == 1) {
+        v[0] = bf16_value(*p);
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        v[0] = bf16_low(a.x); v[1] = bf16_high(a.x); v[2] = bf16_low(a.y); v[3] = bf16_high(a.y);
+        v[4] = bf16_low(a.z); v[5] = bf16_high(a.z); v[6] = bf16_low(a.w); v[7] = bf16_high(a.w);
+    }
+}
+template <int kVec>
+__device__ __forceinline__ void store_group(float* p, const float (&v)[kVec]) {
+    if constexpr (kVec == 1) {
+        *p = v[0];
+    } else {
+        store_f4(p, make_float4(v[0], v[1], v[2], v[3]));
+        store_f4(p + 4, make_float4(v[4], v[5], v[6], v[7]));
+    }
+}
+template <int kVec>
+__device__ __forceinline__ void store_group(unsigned short* p, const float (&v)[kVec]) {
+    if constexpr (kVec == 1) {
+        *p = bf16_bits(v[0]);
+    } else {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]),
+                                                  pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    }
+}
+__device__ __forceinline__ float load_weight(const void* weight, int kind, long long i) {
+    return kind == 0 ? static_cast<const float*>(weight)[i] : bf16_value(static_cast<const unsigned short*>(weight)[i]);
+}
+
+// ---- forward ------------------------------------------------------------------
+
+struct ForwardArguments {
+    const void* x;
+    const void* residual;              // null: h = x
+    const void* weight;
+    void* residual_out;                // null: h is not stored
+    void* y;                           // null, or y (no payload) / the decode of the payload
+    signed char* payload;              // null: not encoded
+    float* scales;
+    float* inverse_rms;                // null: not stored
+    int* finite_status;                // null: not raised
+    long long rows, x_stride, residual_stride;
+    int width, block, weight_kind, y_kind;
+    float epsilon;
+};
+
+__device__ __forceinline__ float inverse_of(float squares, int width, float epsilon, bool& bad) {
+    const float mean = __fdiv_rn(squares, static_cast<float>(width));
+    bad |= is_non_finite(mean);
+    return __frsqrt_rn(__fadd_rn(mean, epsilon));
+}
+
+template <int kVec>
+__device__ __forceinline__ void store_y(void* y, int kind, long long at, const float (&v)[kVec]) {
+    if (kind == 0) store_group<kVec>(static_cast<float*>(y) + at, v);
+    else store_group<kVec>(static_cast<unsigned short*>(y) + at, v);
+}
+
+// Codes of a group against its block's scale: payload, and the values that the
+// codes stand for.
+template <int kVec>
+__device__ __forceinline__ void encode_group(float (&y)[kVec], float scale, signed char* payload) {
+    const BlockScale divisor = block_scale(scale);
+    if constexpr (kVec == 1) {
+        const float t = biased_code_of(y[0], divisor);
+        *payload = code_byte(t);
+        y[0] = __fmul_rn(code_value(t), scale);
+    } else {
+        float t[8];
+        biased_codes_of(make_float4(y[0], y[1], y[2], y[3]), divisor, t[0], t[1], t[2], t[3]);
+        biased_codes_of(make_float4(y[4], y[5], y[6], y[7]), divisor, t[4], t[5], t[6], t[7]);
+        *reinterpret_cast<uint2*>(payload) = make_uint2(pack_codes(t[0], t[1], t[2], t[3]), pack_codes(t[4], t[5], t[6], t[7]));
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(code_value(t[i]), scale);
+    }
+}
+
+// kBlock: -1 = no encode, 0 = one scale a row, else the block size; a block is
+// kBlock / kVec neighbouring lanes of a warp.
+template <typename T, int kVec, int kGroups, int kBlock>
+__global__ void __launch_bounds__(kRowThreads)
+rms_norm_forward_kernel(ForwardArguments a) {
+    __shared__ float slots[2][kRowThreads / 32];
+    RowSum sums{slots, 0};
+    const int threads = blockDim.x;
+    float w[kGroups][kVec];
+    #pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        const int column = (g * threads + threadIdx.x) * kVec;
+        #pragma unroll
+        for (int i = 0; i < kVec; ++i) w[g][i] = column < a.width ? load_weight(a.weight, a.weight_kind, column + i) : 0.0f;
+    }
+    bool bad = false;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+        const long long base = row * a.width;
+        float h[kGroups][kVec];
+        #pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            const int column = (g * threads + threadIdx.x) * kVec;
+            if (column < a.width) {
+                load_group<kVec>(x + column, h[g]);
+            } else {
+                #pragma unroll
+                for (int i = 0; i < kVec; ++i) h[g][i] = 0.0f;
+            }
+        }
+        if (a.residual != nullptr) {
+            const T* residual = static_cast<const T*>(a.residual) + row * a.residual_stride;
+            #pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                const int column = (g * threads + threadIdx.x) * kVec;
+                if (column < a.width) {
+                    float r[kVec];
+                    load_group<kVec>(residual + column, r);
+                    #pragma unroll
+                    for (int i = 0; i < kVec; ++i) h[g][i] = __fadd_rn(h[g][i], r[i]);
+                }
+            }
+        }
+        float squares = 0.0f;
+        #pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            const int column = (g * threads + threadIdx.x) * kVec;
+            if (a.residual_out != nullptr && column < a.width)
+                store_group<kVec>(static_cast<T*>(a.residual_out) + base + column, h[g]);
+            #pragma unroll
+            for (int i = 0; i < kVec; ++i) squares = __fmaf_rn(h[g][i], h[g][i], squares);
+        }
+        const float inverse = inverse_of(over_cta<false>(squares, sums), a.width, a.epsilon, bad);
+        if (a.inverse_rms != nullptr && threadIdx.x == 0) a.inverse_rms[row] = inverse;
+        float largest = 0.0f;
+        #pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            #pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                h[g][i] = __fmul_rn(__fmul_rn(h[g][i], inverse), w[g][i]);
+                bad |= is_non_finite(h[g][i]);
+                if (kBlock == 0) largest = fmaxf(largest, fabsf(h[g][i]));
+            }
+        }
+        float row_scale = 1.0f;
+        if constexpr (kBlock == 0) {
+            row_scale = scale_from_maximum_fast(over_cta<true>(largest, sums));
+            if (threadIdx.x == 0) a.scales[row] = row_scale;
+        }
+        #pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            const int column = (g * threads + threadIdx.x) * kVec;
+            if constexpr (kBlock > 0) {
+                constexpr int kLanes = kBlock / kVec;
+                float maximum = 0.0f;
+                #pragma unroll
+                for (int i = 0; i < kVec; ++i) maximum = fmaxf(maximum, fabsf(h[g][i]));
+                const float scale = scale_from_maximum_fast(group_max<kLanes>(maximum));
+                if (column < a.width) {
+                    if (threadIdx.x % kLanes == 0) a.scales[(base + column) / kBlock] = scale;
+                    encode_group<kVec>(h[g], scale, a.payload + base + column);
+                }
+            } else if constexpr (kBlock == 0) {
+                if (column < a.width) encode_group<kVec>(h[g], row_scale, a.payload + base + column);
+            }
+            if (a.y != nullptr && column < a.width) store_y<kVec>(a.y, a.y_kind, base + column, h[g]);
+        }
+    }
+    if (a.finite_status != nullptr && __any_sync(0xffffffffu, bad) && (threadIdx.x & 31) == 0)
+        atomicExch(a.finite_status, 1);
+}
+
+// Any width, any block size that divides it, any alignment: the row is read
+// once for its sum of squares, (one scale a row: once more for its maximum,)
+// and then block by block, a warp to a block, for the maximum and the codes.
+// h may be stored over x or the residual, so it is stored by the last pass,
+// by the thread that reads the value there.
+template <typename T>
+__global__ void __launch_bounds__(kLoopThreads)
+rms_norm_forward_loop_kernel(ForwardArguments a) {
+    __shared__ float slots[2][kRowThreads / 32];
+    RowSum sums{slots, 0};
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kLoopThreads / 32;
+    bool bad = false;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+        const T* residual = a.residual == nullptr ? nullptr : static_cast<const T*>(a.residual) + row * a.residual_stride;
+        const long long base = row * a.width;
+        auto h_at = [&](int i) {
+            float v[1];
+            load_group<1>(x + i, v);
+            if (residual != nullptr) {
+                float r[1];
+                load_group<1>(residual + i, r);
+                v[0] = __fadd_rn(v[0], r[0]);
+            }
+            return v[0];
+        };
+        float squares = 0.0f;
+        for (int i = threadIdx.x; i < a.width; i += kLoopThreads) {
+            const float h = h_at(i);
+            squares = __fmaf_rn(h, h, squares);
+        }
+        const float inverse = inverse_of(over_cta<false>(squares, sums), a.width, a.epsilon, bad);
+        if (a.inverse_rms != nullptr && threadIdx.x == 0) a.inverse_rms[row] = inverse;
+        auto y_of = [&](float h, int i) {
+            return __fmul_rn(__fmul_rn(h, inverse), load_weight(a.weight, a.weight_kind, i));
+        };
+        auto finish = [&](int i, float scale) {
+            float h[1] = {h_at(i)};
+            float y[1] = {y_of(h[0], i)};
+            bad |= is_non_finite(y[0]);
+            if (a.payload != nullptr) encode_group<1>(y, scale, a.payload + base + i);
+            if (a.residual_out != nullptr) store_group<1>(static_cast<T*>(a.residual_out) + base + i, h);
+            if (a.y != nullptr) store_y<1>(a.y, a.y_kind, base + i, y);
+        };
+        if (a.payload == nullptr || a.block == a.width) {
+            float scale = 1.0f;
+            if (a.payload != nullptr) {
+                float largest = 0.0f;
+                for (int i = threadIdx.x; i < a.width; i += kLoopThreads) largest = fmaxf(largest, fabsf(y_of(h_at(i), i)));
+                scale = scale_from_maximum_fast(over_cta<true>(largest, sums));
+                if (threadIdx.x == 0) a.scales[row] = scale;
+            }
+            for (int i = threadIdx.x; i < a.width; i += kLoopThreads) finish(i, scale);
+            continue;
+        }
+        const int blocks = a.width / a.block;
+        for (int b = warp; b < blocks; b += warps) {
+            float largest = 0.0f;
+            for (int i = b * a.block + lane; i < (b + 1) * a.block; i += 32) largest = fmaxf(largest, fabsf(y_of(h_at(i), i)));
+            const float scale = scale_from_maximum_fast(group_max<32>(largest));
+            if (lane == 0) a.scales[row * blocks + b] = scale;
+            for (int i = b * a.block + lane; i < (b + 1) * a.block; i += 32) finish(i, scale);
+        }
+    }
+    if (a.finite_status != nullptr && __any_sync(0xffffffffu, bad) && lane == 0) atomicExch(a.finite_status, 1);
+}
+
+// ---- backward -----------------------------------------------------------------
+
+struct BackwardArguments {
+    const void* y_gradient;
+    const void* residual_gradient;     // null: nothing is added to dx
+    const void* h;
+    const void* weight;
+    const float* inverse_rms;
+    void* x_gradient;
+    float* partials;                   // [CTAs][width]
+    long long rows, y_stride, residual_stride, h_stride;
+    int width, weight_kind;
+};
+
+template <typename T, int kVec, int kGroups>
+__global__ void __launch_bounds__(kRowThreads)
+rms_norm_backward_kernel(BackwardArguments a) {
+    __shared__ float slots[2][kRowThreads / 32];
+    RowSum sums{slots, 0};
+    const int threads = blockDim.x;
+    float w[kGroups][kVec], dw[kGroups][kVec];
+    #pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        const int column = (g * threads + threadIdx.x) * kVec;
+        #pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            w[g][i] = column < a.width ? load_weight(a.weight, a.weight_kind, column + i) : 0.0f;
+            dw[g][i] = 0.0f;
+        }
+    }
+    const float width = static_cast<float>(a.width);
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* dy = static_cast<const T*>(a.y_gradient) + row * a.y_stride;
+        const T* h = static_cast<const T*>(a.h) + row * a.h_stride;
+        const float inverse = a.inverse_rms[row];
+        float d[kGroups][kVec], n[kGroups][kVec];
+        #pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            const int column = (g * threads + threadIdx.x) * kVec;
+            if (column < a.width) {
+                load_group<kVec>(dy + column, d[g]);
+                load_group<kVec>(h + column, n[g]);
+            } else {
+                #pragma unroll
+                for (int i = 0; i < kVec; ++i) d[g][i] = n[g][i] = 0.0f;
+            }
+        }
+        float along = 0.0f;
+        #pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            #pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                n[g][i] = __fmul_rn(n[g][i], inverse);
+                dw[g][i] = __fmaf_rn(d[g][i], n[g][i], dw[g][i]);
+                d[g][i] = __fmul_rn(d[g][i], w[g][i]);
+                along = __fmaf_rn(d[g][i], n[g][i], along);
+            }
+        }
+        const float mean = __fdiv_rn(over_cta<false>(along, sums), width);
+        #pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            const int column = (g * threads + threadIdx.x) * kVec;
+            if (column >= a.width) continue;
+            float r[kVec];
+            if (a.residual_gradient != nullptr) {
+                load_group<kVec>(static_cast<const T*>(a.residual_gradient) + row * a.residual_stride + column, r);
+            } else {
+                #pragma unroll
+                for (int i = 0; i < kVec; ++i) r[i] = 0.0f;
+            }
+            #pragma unroll
+            for (int i = 0; i < kVec; ++i) d[g][i] = __fmaf_rn(inverse, __fmaf_rn(-n[g][i], mean, d[g][i]), r[i]);
+            store_group<kVec>(static_cast<T*>(a.x_gradient) + row * a.width + column, d[g]);
+        }
+    }
+    float* partial = a.partials + static_cast<long long>(blockIdx.x) * a.width;
+    #pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        const int column = (g * threads + threadIdx.x) * kVec;
+        #pragma unroll
+        for (int i = 0; i < kVec; ++i)
+            if (column < a.width) partial[column + i] = dw[g][i];
+    }
+}
+
+// Any width and alignment: the row is read twice, the partial weight gradient
+// is kept in memory; a thread always has the same columns.
+template <typename T>
+__global__ void __launch_bounds__(kLoopThreads)
+rms_norm_backward_loop_kernel(BackwardArguments a) {
+    __shared__ float slots[2][kRowThreads / 32];
+    RowSum sums{slots, 0};
+    float* partial = a.partials + static_cast<long long>(blockIdx.x) * a.width;
+    for (int i = threadIdx.x; i < a.width; i += kLoopThreads) partial[i] = 0.0f;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* dy = static_cast<const T*>(a.y_gradient) + row * a.y_stride;
+        const T* h = static_cast<const T*>(a.h) + row * a.h_stride;
+        const float inverse = a.inverse_rms[row];
+        float along = 0.0f;
+        for (int i = threadIdx.x; i < a.width; i += kLoopThreads) {
+            float d[1], n[1];
+            load_group<1>(dy + i, d);
+            load_group<1>(h + i, n);
+            n[0] = __fmul_rn(n[0], inverse);
+            partial[i] = __fmaf_rn(d[0], n[0], partial[i]);
+            along = __fmaf_rn(__fmul_rn(d[0], load_weight(a.weight, a.weight_kind, i)), n[0], along);
+        }
+        const float mean = __fdiv_rn(over_cta<false>(along, sums), static_cast<float>(a.width));
+        for (int i = threadIdx.x; i < a.width; i += kLoopThreads) {
+            float d[1], n[1], r[1] = {0.0f};
+            load_group<1>(dy + i, d);
+            load_group<1>(h + i, n);
+            if (a.residual_gradient != nullptr)
+                load_group<1>(static_cast<const T*>(a.residual_gradient) + row * a.residual_stride + i, r);
+            const float g = __fmul_rn(d[0], load_weight(a.weight, a.weight_kind, i));
+            d[0] = __fmaf_rn(inverse, __fmaf_rn(-__fmul_rn(n[0], inverse), mean, g), r[0]);
+            store_group<1>(static_cast<T*>(a.x_gradient) + row * a.width + i, d);
+        }
+    }
+}
+
+// dw (+)= sum of the partials, in a fixed order: 32 threads share a column.
+__global__ void __launch_bounds__(kJoinColumns * kJoinRows)
+rms_norm_join_kernel(const float* partials, int count, int width, void* weight_gradient, int kind, bool accumulate) {
+    __shared__ float sums[kJoinRows][kJoinColumns + 1];
+    const int x = threadIdx.x % kJoinColumns, y = threadIdx.x / kJoinColumns;
+    const int column = blockIdx.x * kJoinColumns + x;
+    wait_for_previous();
+    float sum = 0.0f;
+    if (column < width) {
+        #pragma unroll 8
+        for (int r = y; r < count; r += kJoinRows) sum = __fadd_rn(sum, partials[static_cast<long long>(r) * width + column]);
+    }
+    sums[y][x] = sum;
+    __syncthreads();
+    // warp y sums column y of the tile over its 32 rows
+    float total = sums[x][y];
+    #pragma unroll
+    for (int offset = 16; offset > 0; offset >>= 1) total = __fadd_rn(total, __shfl_xor_sync(0xffffffffu, total, offset));
+    const int mine = blockIdx.x * kJoinColumns + y;
+    if (x != 0 || mine >= width) return;
+    if (kind == 0) {
+        float* out = static_cast<float*>(weight_gradient) + mine;
+        *out = accumulate ? __fadd_rn(*out, total) : total;
+    } else {
+        unsigned short* out = static_cast<unsigned short*>(weight_gradient) + mine;
+        *out = bf16_bits(accumulate ? __fadd_rn(bf16_value(*out), total) : total);
+    }
+}
+
+// ---- launch shapes ---------------------------------------------------------------
+
+// One resident wave of kKernel with `threads` threads.
+template <auto kKernel>
+int resident_grid(int threads, long long rows) {
+    static std::atomic<int> known[kRowThreads / 32 + 1];
+    std::atomic<int>& slot = known[threads / 32];
+    int fit = slot.load(std::memory_order_relaxed);
+    if (fit == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kKernel, threads, 0) != cudaSuccess || fit < 1) fit = 1;
+        slot.store(fit, std::memory_order_relaxed);
+    }
+    return grid_for(rows, fit);
+}
+
+struct RowShape {
+    int groups, threads;               // groups 0: the row does not fit registers
+};
+
+// Threads and groups per thread for a row of `units` groups of 8 values: the
+// fewest groups that keep a row within 256 threads, so several rows share an SM
+// and their barriers overlap; few rows (fewer than SMs) get more threads each.
+int threads_for(int units, int groups) { return ((units + groups - 1) / groups + 31) / 32 * 32; }
+
+RowShape row_shape(int units, long long rows) {
+    const int want = rows < sm_count() ? kRowThreads : 256;
+    for (int groups = 1; groups <= 4; groups *= 2) {
+        const int threads = threads_for(units, groups);
+        if (threads <= want || (groups == 4 && threads <= kRowThreads)) return {groups, threads};
+    }
+    return {0, 0};
+}
+
+template <typename T, int kVec, int kGroups, int kBlock>
+cudaError_t launch_forward(const ForwardArguments& a, int threads, cudaStream_t stream) {
+    constexpr auto kKernel = rms_norm_forward_kernel<T, kVec, kGroups, kBlock>;
+    kKernel<<<resident_grid<kKernel>(threads, a.rows), threads, 0, stream>>>(a);
+    return cudaPeekAtLastError();
+}
+
+template <typename T, int kVec, int kGroups>
+cudaError_t forward_by_block(const ForwardArguments& a, int threads, cudaStream_t stream) {
+    if (a.payload == nullptr) return launch_forward<T, kVec, kGroups, -1>(a, threads, stream);
+    if (a.block == a.width) return launch_forward<T, kVec, kGroups, 0>(a, threads, stream);
+    if (a.block == 32) return launch_forward<T, kVec, kGroups, 32>(a, threads, stream);
+    if constexpr (kVec == 8) {
+        if (a.block == 64) return launch_forward<T, kVec, kGroups, 64>(a, threads, stream);
+        return launch_forward<T, kVec, kGroups, 128>(a, threads, stream);
+    }
+    return cudaErrorInvalidValue;
+}
+
+template <typename T>
+cudaError_t run_forward(const ForwardArguments& a, bool vector_ok, cudaStream_t stream) {
+    const bool whole = a.payload == nullptr || a.block == a.width;
+    if (vector_ok && (whole || a.block == 32 || a.block == 64 || a.block == 128)) {
+        const RowShape s = row_shape(a.width / 8, a.rows);
+        if (s.groups == 1) return forward_by_block<T, 8, 1>(a, s.threads, stream);
+        if (s.groups == 2) return forward_by_block<T, 8, 2>(a, s.threads, stream);
+        if (s.groups == 4) return forward_by_block<T, 8, 4>(a, s.threads, stream);
+    } else if (whole || a.block == 32) {
+        if (a.width <= 4 * kRowThreads) return forward_by_block<T, 1, 4>(a, threads_for(a.width, 4), stream);
+        if (a.width <= 16 * kRowThreads) return forward_by_block<T, 1, 16>(a, threads_for(a.width, 16), stream);
+    }
+    constexpr auto kKernel = rms_norm_forward_loop_kernel<T>;
+    kKernel<<<resident_grid<kKernel>(kLoopThreads, a.rows), kLoopThreads, 0, stream>>>(a);
+    return cudaPeekAtLastError();
+}
+
+template <typename T, int kVec, int kGroups>
+cudaError_t launch_backward(const BackwardArguments& a, int threads, int& grid, cudaStream_t stream) {
+    constexpr auto kKernel = rms_norm_backward_kernel<T, kVec, kGroups>;
+    grid = resident_grid<kKernel>(threads, a.rows);
+    if (grid > kMostPartials) grid = kMostPartials;
+    kKernel<<<grid, threads, 0, stream>>>(a);
+    return cudaPeekAtLastError();
+}
+
+template <typename T>
+cudaError_t run_backward(const BackwardArguments& a, bool vector_ok, int& grid, cudaStream_t stream) {
+    if (vector_ok) {
+        const RowShape s = row_shape(a.width / 8, a.rows);
+        if (s.groups == 1) return launch_backward<T, 8, 1>(a, s.threads, grid, stream);
+        if (s.groups == 2) return launch_backward<T, 8, 2>(a, s.threads, grid, stream);
+        if (s.groups == 4) return launch_backward<T, 8, 4>(a, s.threads, grid, stream);
+    } else {
+        if (a.width <= 4 * kRowThreads) return launch_backward<T, 1, 4>(a, threads_for(a.width, 4), grid, stream);
+        if (a.width <= 16 * kRowThreads) return launch_backward<T, 1, 16>(a, threads_for(a.width, 16), grid, stream);
+    }
+    constexpr auto kKernel = rms_norm_backward_loop_kernel<T>;
+    grid = resident_grid<kKernel>(kLoopThreads, a.rows);
+    if (grid > kMostPartials) grid = kMostPartials;
+    kKernel<<<grid, kLoopThreads, 0, stream>>>(a);
+    return cudaPeekAtLastError();
+}
+
+// Rows of `kind` at `p`, `stride` values apart: 128-bit accesses possible?
+bool rows_aligned(const void* p, int kind, long long stride) {
+    return aligned_for(p, 16) && stride * (kind == 0 ? 4 : 2) % 16 == 0;
+}
+bool typed(const void* p, int kind) { return aligned_for(p, kind == 0 ? 4 : 2); }
+bool is_kind(int kind) { return kind == 0 || kind == 1; }
+
+constexpr long long kMostRows = 1ll << 40;
+constexpr int kMostWidth = 1 << 24;
+long long partial_count(long long rows) { return rows < kMostPartials ? rows : kMostPartials; }
+
+int forward(int device, int kind, const void* x, long long x_stride, const void* residual, long long residual_stride,
+            const void* weight, int weight_kind, long long rows, int width, float epsilon, void* residual_out, void* y,
+            int y_kind, signed char* payload, float* scales, int block_size, float* inverse_rms, int* finite_status,
+            cudaStream_t stream) {
+    if (!is_kind(kind) || !is_kind(weight_kind) || !is_kind(y_kind) || rows < 0 || rows > kMostRows || width < 1 ||
+        width > kMostWidth || block_size < 0 || !(epsilon >= 0.0f) || std::isinf(epsilon) || x_stride < width ||
+        (residual && residual_stride < width))
+        return static_cast<int>(cudaErrorInvalidValue);
+    const int block = block_size == 0 || block_size > width ? width : block_size;
+    if (!weight || (rows > 0 && !y && !payload) || (payload && (!scales || width % block != 0)) || (residual_out && !residual) ||
+        (rows > 0 && !x) || !typed(x, kind) || !typed(residual, kind) || !typed(weight, weight_kind) ||
+        !typed(residual_out, kind) || !typed(y, y_kind) || !aligned_for(scales, 4) || !aligned_for(inverse_rms, 4) ||
+        !aligned_for(finite_status, 4))
+        return static_cast<int>(cudaErrorInvalidValue);
+    if (rows == 0) return static_cast<int>(cudaSuccess);
+    const DeviceScope scope(device);
+    if (scope.status() != cudaSuccess) return scope.status();
+    const ForwardArguments a{x, residual, weight, residual_out, y, payload, scales, inverse_rms, finite_status,
+                             rows, x_stride, residual_stride, width, block, weight_kind, y_kind, epsilon};
+    const bool vector_ok = width % 8 == 0 && rows_aligned(x, kind, x_stride) &&
+                           (!residual || rows_aligned(residual, kind, residual_stride)) &&
+                           aligned_for(residual_out, 16) && aligned_for(y, 16) && aligned_for(payload, 8);
+    return static_cast<int>(kind == 0 ? run_forward<float>(a, vector_ok, stream)
+                                      : run_forward<unsigned short>(a, vector_ok, stream));
+}
+
+int backward(int device, int kind, const void* y_gradient, long long y_stride, const void* residual_gradient,
+             long long residual_stride, const void* h, long long h_stride, const void* weight, int weight_kind,
+             const float* inverse_rms, long long rows, int width, void* x_gradient, void* weight_gradient,
+             int weight_gradient_kind, int accumulate, void* workspace, long long workspace_bytes, cudaStream_t stream) {
+    if (!is_kind(kind) || !is_kind(weight_kind) || !is_kind(weight_gradient_kind) || rows < 0 || rows > kMostRows ||
+        width < 1 || width > kMostWidth || y_stride < width || h_stride < width ||
+        (residual_gradient && residual_stride < width))
+        return static_cast<int>(cudaErrorInvalidValue);
+    if (!weight || !weight_gradient || (rows > 0 && (!y_gradient || !h || !inverse_rms || !x_gradient || !workspace)) ||
+        !typed(y_gradient, kind) || !typed(residual_gradient, kind) || !typed(h, kind) || !typed(x_gradient, kind) ||
+        !typed(weight, weight_kind) || !typed(weight_gradient, weight_gradient_kind) || !aligned_for(inverse_rms, 4) ||
+        !aligned_for(workspace, 4) || workspace_bytes < partial_count(rows) * width * 4)
+        return static_cast<int>(cudaErrorInvalidValue);
+    const DeviceScope scope(device);
+    if (scope.status() != cudaSuccess) return scope.status();
+    int grid = 0;
+    cudaError_t e = cudaSuccess;
+    if (rows > 0) {
+        const BackwardArguments a{y_gradient, residual_gradient, h, weight, inverse_rms, x_gradient,
+                                  static_cast<float*>(workspace), rows, y_stride, residual_stride, h_stride, width, weight_kind};
+        const bool vector_ok = width % 8 == 0 && rows_aligned(y_gradient, kind, y_stride) && rows_aligned(h, kind, h_stride) &&
+                               (!residual_gradient || rows_aligned(residual_gradient, kind, residual_stride)) &&
+                               aligned_for(x_gradient, 16);
+        e = kind == 0 ? run_backward<float>(a, vector_ok, grid, stream) : run_backward<unsigned short>(a, vector_ok, grid, stream);
+    }
+    if (e == cudaSuccess)
+        e = launch_dependent(rms_norm_join_kernel, (width + kJoinColumns - 1) / kJoinColumns, kJoinColumns * kJoinRows, 0,
+                             stream, static_cast<const float*>(workspace), grid, width, weight_gradient,
+                             weight_gradient_kind, accumulate != 0);
+    return static_cast<int>(e);
+}
+
+}  // namespace
+}  // namespace ngb
+
+using namespace ngb;
+
+NNTRAIN_EXPORT int nntrain_rms_norm_forward(
+    int device, int kind, const void* x, long long x_stride, const void* residual, long long residual_stride,
+    const void* weight, int weight_kind, long long rows, int width, float epsilon, void* residual_out, void* y, int y_kind,
+    signed char* payload, float* scales, int block_size, float* inverse_rms, int* finite_status, nntrain_stream_t stream) {
+    return complete(kOpRmsNorm, device,
+                    forward(device, kind, x, x_stride, residual, residual_stride, weight, weight_kind, rows, width, epsilon,
+                            residual_out, y, y_kind, payload, scales, block_size, inverse_rms, finite_status,
+                            static_cast<cudaStream_t>(stream)));
+}
+
+NNTRAIN_EXPORT int nntrain_rms_norm_backward_workspace(long long rows, int width, long long* bytes) {
+    if (rows < 0 || rows > kMostRows || width < 1 || width > kMostWidth || !bytes)
+        return complete(kOpRmsNorm, -1, static_cast<int>(cudaErrorInvalidValue));
+    *bytes = partial_count(rows) * width * 4;
+    return static_cast<int>(cudaSuccess);
+}
+
+NNTRAIN_EXPORT int nntrain_rms_norm_backward(
+    int device, int kind, const void* y_gradient, long long y_stride, const void* residual_gradient,
+    long long residual_stride, const void* h, long long h_stride, const void* weight, int weight_kind,
+    const float* inverse_rms, long long rows, int width, void* x_gradient, void* weight_gradient, int weight_gradient_kind,
+    int accumulate, void* workspace, long long workspace_bytes, nntrain_stream_t stream) {
+    return complete(kOpRmsNorm, device,
+                    backward(device, kind, y_gradient, y_stride, residual_gradient, residual_stride, h, h_stride, weight,
+                             weight_kind, inverse_rms, rows, width, x_gradient, weight_gradient, weight_gradient_kind,
+                             accumulate, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)));
+}

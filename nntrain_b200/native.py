@@ -9,6 +9,7 @@ buffers.
   CudaGradientBuckets     NNtrain.Core/Tensors/CudaGradientBuckets.cs:6-349
   GradientNorm            the norm / clip kernels behind
                           NNtrain.Core/Tensors/Tensor.CudaKernels.cs:119-854
+  RmsNorm                 root-mean-square norm with an encoded output, and its gradient
   GradientTensorList      the leaves that clip_grad_norm_ walks there, as one
                           table (NNtrain.Core/Torch/nn.cs:32-81)
 """
@@ -72,6 +73,18 @@ def _scratch(device: int, bytes_: int, stream):
         stream = torch.cuda.ExternalStream(stream, device=device)
     with torch.cuda.stream(stream):
         return torch.empty(bytes_, dtype=torch.uint8, device=torch.device("cuda", device))
+
+
+def _workspace(operation: str, bytes_of, sizes, device: int, given, stream):
+    """(scratch, its bytes) for one call: the caller's, or allocated for it."""
+    need = ctypes.c_longlong()
+    check(operation, bytes_of(*sizes, ctypes.addressof(need)))
+    if given is None:
+        return _scratch(device, need.value, stream), need.value
+    _require(given, torch.uint8, "workspace", device)
+    if given.numel() < need.value:
+        raise ValueError(f"workspace has {given.numel()} bytes, needs {need.value}")
+    return given, given.numel()
 
 
 def scale_count(length: int, block_size: int) -> int:
@@ -486,3 +499,100 @@ class Bfp8GradientOptimizers:
             device, _ptr(data), _ptr(gradient_payload), _ptr(gradient_scales), block_size, _ptr(first_moment),
             _ptr(second_moment), _ptr(compute_bf16), n, beta1, beta2, learning_rate, weight_decay, update_scale,
             scaled_epsilon, int(apply_weight_decay), _stream(stream)))
+
+
+def _rows(t: torch.Tensor, name: str, device: int, width: int, dtypes, rows: int | None = None) -> int:
+    """Checks a matrix of rows (contiguous values, any row stride) and returns the stride."""
+    if not t.is_cuda or t.device.index != device:
+        raise ValueError(f"{name} must be on CUDA device {device}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} has type {t.dtype}, expected one of {', '.join(map(str, dtypes))}")
+    if t.dim() != 2 or t.shape[1] != width or (rows is not None and t.shape[0] != rows):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({'rows' if rows is None else rows}, {width})")
+    if t.shape[0] <= 1:
+        if width > 1 and t.shape[0] == 1 and t.stride(1) != 1:
+            raise ValueError(f"{name}: the values of a row must be contiguous")
+        return width
+    if (width > 1 and t.stride(1) != 1) or t.stride(0) < width:
+        raise ValueError(f"{name}: the values of a row must be contiguous and rows must not overlap")
+    return t.stride(0)
+
+
+def _vector(t: torch.Tensor, name: str, device: int, length: int, dtypes) -> None:
+    _require(t, t.dtype, name, device)
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} has type {t.dtype}, expected one of {', '.join(map(str, dtypes))}")
+    if t.numel() != length:
+        raise ValueError(f"{name} has {t.numel()} values, expected {length}")
+
+
+class RmsNorm:
+    """Root-mean-square norm of x + residual whose output goes to the codec's 8
+    bits, and its gradient.  Matrices are (rows, width), fp32 or bf16 (bfloat16
+    or its bits); inputs may have any row stride, outputs are contiguous."""
+
+    @staticmethod
+    def forward(device: int, x, weight, epsilon: float, residual=None, residual_out=None, y=None, payload=None,
+                scales=None, block_size: int = 0, inverse_rms=None, finite_status=None, stream=None) -> None:
+        """h = x + residual, i = 1 / sqrt(mean(h^2) + epsilon), y = h * i * weight.
+        `payload` and `scales`: y encoded, `block_size` values to a scale (a divisor
+        of the width; 0 = one scale a row).  `y` (fp32 or bf16): y itself, or with a
+        payload the values that the codes stand for.  `residual_out`: h, in x's
+        type (x or residual itself is allowed); `inverse_rms`: i for the gradient."""
+        if x.dim() != 2:
+            raise ValueError(f"x has shape {tuple(x.shape)}, expected (rows, width)")
+        rows, width = x.shape
+        same = _FLOAT32 if x.dtype == torch.float32 else _BFLOAT16
+        x_stride = _rows(x, "x", device, width, same)
+        residual_stride = 0 if residual is None else _rows(residual, "residual", device, width, same, rows)
+        _vector(weight, "weight", device, width, _FLOATS)
+        if y is None and payload is None:
+            raise ValueError("the norm needs an output: y, or payload and scales")
+        if y is not None:
+            _vector(y, "y", device, rows * width, _FLOATS)
+        if residual_out is not None:
+            if residual is None:
+                raise ValueError("residual_out without a residual is x itself")
+            _vector(residual_out, "residual_out", device, rows * width, same)
+        if payload is not None:
+            block = width if block_size == 0 or block_size > width else block_size
+            if block < 0 or scales is None or (width and width % block != 0):
+                raise ValueError("an encoded output needs scales and a block size that divides the width")
+            _vector(payload, "payload", device, rows * width, (torch.int8,))
+            _vector(scales, "scales", device, rows * (width // block) if width else 0, _FLOAT32)
+        if inverse_rms is not None:
+            _vector(inverse_rms, "inverse_rms", device, rows, _FLOAT32)
+        if finite_status is not None:
+            _require(finite_status, torch.int32, "finite_status", device)
+        check("rms_norm_forward", load().nntrain_rms_norm_forward(
+            device, _kind(x), x.data_ptr(), x_stride, _ptr(residual), residual_stride, weight.data_ptr(), _kind(weight),
+            rows, width, epsilon, _ptr(residual_out), _ptr(y), 0 if y is None else _kind(y), _ptr(payload), _ptr(scales),
+            block_size, _ptr(inverse_rms), _ptr(finite_status), _stream_on(device, stream)))
+
+    @staticmethod
+    def backward(device: int, y_gradient, h, weight, inverse_rms, x_gradient, weight_gradient, residual_gradient=None,
+                 accumulate: bool = False, workspace=None, stream=None) -> None:
+        """From the gradient of y, h = x + residual (what `residual_out` holds, or x)
+        and `inverse_rms`: `x_gradient`, the gradient of x and of residual alike,
+        plus `residual_gradient`, what reaches h from elsewhere; and
+        `weight_gradient` (fp32 or bf16), added to what is there with `accumulate`.
+        x_gradient may be y_gradient or residual_gradient itself.  `workspace`
+        (optional): uint8 scratch that no call in flight at the same time uses."""
+        if h.dim() != 2:
+            raise ValueError(f"h has shape {tuple(h.shape)}, expected (rows, width)")
+        rows, width = h.shape
+        same = _FLOAT32 if h.dtype == torch.float32 else _BFLOAT16
+        h_stride = _rows(h, "h", device, width, same)
+        y_stride = _rows(y_gradient, "y_gradient", device, width, same, rows)
+        residual_stride = 0 if residual_gradient is None else _rows(residual_gradient, "residual_gradient", device, width, same, rows)
+        _vector(weight, "weight", device, width, _FLOATS)
+        _vector(inverse_rms, "inverse_rms", device, rows, _FLOAT32)
+        _vector(x_gradient, "x_gradient", device, rows * width, same)
+        _vector(weight_gradient, "weight_gradient", device, width, _FLOATS)
+        workspace, bytes_ = _workspace("rms_norm_backward", load().nntrain_rms_norm_backward_workspace, (rows, width), device,
+                                       workspace, stream)
+        check("rms_norm_backward", load().nntrain_rms_norm_backward(
+            device, _kind(h), y_gradient.data_ptr(), y_stride, _ptr(residual_gradient), residual_stride, h.data_ptr(),
+            h_stride, weight.data_ptr(), _kind(weight), inverse_rms.data_ptr(), rows, width, x_gradient.data_ptr(),
+            weight_gradient.data_ptr(), _kind(weight_gradient), int(accumulate), _ptr(workspace), bytes_,
+            _stream_on(device, stream)))
