@@ -377,6 +377,39 @@ int nntrain_rms_norm_backward(
     int weight_gradient_kind, int accumulate, void* workspace, long long workspace_bytes,
     nntrain_stream_t stream);
 
+/* ---- token table (ABI minor 36; no counterpart in the reference's gradient
+ * path) ------------------------------------------------------------------------
+ * table_kind: 0 = fp32, 1 = bf16, 2 = BFP8 (lookup only); out_kind,
+ * gradient_kind: 0 = fp32, 1 = bf16.  tokens: `count` row numbers of
+ * token_bytes (4 or 8) each.  padding_token (any value) is no token; a token
+ * that is neither it nor a row of the table is none either, and sets
+ * *token_status (optional) to 1.  Addresses need the alignment of their type
+ * only. */
+
+/* out[t] = scale * table[tokens[t]], zeros where there is no token.  A BFP8
+ * table is rows of an encoded arena: value (r, c) has the scale number
+ * (first_value + r * width + c) / block_size (block_size 0 = one scale), so
+ * first_value is the table's place in the arena that `scales` belongs to; it is
+ * decoded in fp32 before the product.  Rows of out lie out_stride values apart. */
+int nntrain_embedding_lookup(
+    int device, int table_kind, const void* table, const float* scales, int block_size,
+    long long first_value, long long vocab, int width, const void* tokens, int token_bytes,
+    long long count, long long padding_token, float scale, int out_kind, void* out,
+    long long out_stride, int* token_status, nntrain_stream_t stream);
+/* Host only: bytes of scratch that nntrain_embedding_gradient needs. */
+int nntrain_embedding_gradient_workspace(long long count, long long vocab, int width, long long* bytes);
+/* table_gradient[v] = scale * sum of out_gradient[t] over the t with
+ * tokens[t] = v: the whole table is written, rows without a token with zeros;
+ * with accumulate != 0 the sums are added to what is there and other rows are
+ * left alone.  fp32 sums in the order of t (32 sorted positions, then their
+ * partials), rounded once: same inputs, same bits.  The scratch (16-byte
+ * aligned) is the caller's, one for each call in flight. */
+int nntrain_embedding_gradient(
+    int device, int gradient_kind, const void* out_gradient, long long gradient_stride,
+    const void* tokens, int token_bytes, long long count, long long padding_token, float scale,
+    int table_kind, void* table_gradient, long long vocab, int width, int accumulate,
+    int* token_status, void* workspace, long long workspace_bytes, nntrain_stream_t stream);
+
 /* ---- N-rank all-reduce, one process per GPU (ABI minor 36) -------------------
  * The reference's compressed reducers accept exactly two devices of one
  * process (NNtrain.Core/Training/CudaBfp8GradientAllReduce.cs:44-49,

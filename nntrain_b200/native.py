@@ -10,6 +10,7 @@ buffers.
   GradientNorm            the norm / clip kernels behind
                           NNtrain.Core/Tensors/Tensor.CudaKernels.cs:119-854
   RmsNorm                 root-mean-square norm with an encoded output, and its gradient
+  TokenEmbedding          rows of a (possibly encoded) token table, and the table's gradient
   GradientTensorList      the leaves that clip_grad_norm_ walks there, as one
                           table (NNtrain.Core/Torch/nn.cs:32-81)
 """
@@ -596,3 +597,74 @@ class RmsNorm:
             h_stride, weight.data_ptr(), _kind(weight), inverse_rms.data_ptr(), rows, width, x_gradient.data_ptr(),
             weight_gradient.data_ptr(), _kind(weight_gradient), int(accumulate), _ptr(workspace), bytes_,
             _stream_on(device, stream)))
+
+
+class TokenEmbedding:
+    """Rows of a token table times a scale, and the table's gradient.  `tokens` are
+    int32 or int64 row numbers, any shape; `padding_token` stands for no token.  A
+    token that is neither it nor a row counts as none and sets `token_status`
+    (optional, int32) to 1."""
+
+    @staticmethod
+    def lookup(device: int, tokens, table, out, scale: float = 1.0, table_scales=None, block_size: int = 0,
+               first_value: int = 0, padding_token: int = -1, token_status=None, stream=None) -> None:
+        """out[t] = scale * table[tokens[t]], zeros where there is no token.  `table`
+        (vocab, width): fp32, bf16 or an int8 payload with the `table_scales` and
+        block size of the arena in which it begins at `first_value`.  `out`
+        (tokens, width): fp32 or bf16, any row stride."""
+        count, bytes_ = _tokens(tokens, device)
+        vocab, width, kind = _table(table, "table", device, _FLOATS + (torch.int8,))
+        out_stride = _rows(out, "out", device, width, _FLOATS, count)
+        if kind == 2:
+            if table_scales is None or block_size < 0 or first_value < 0:
+                raise ValueError("an encoded table needs its scales, block size and place in the arena")
+            _require(table_scales, torch.float32, "table_scales", device)
+            needed = 1 if block_size == 0 else (first_value + vocab * width + block_size - 1) // block_size
+            if table_scales.numel() < needed:
+                raise ValueError(f"table_scales has {table_scales.numel()} values, needs {needed}")
+        elif table_scales is not None:
+            raise ValueError("a table that is not encoded has no scales")
+        if token_status is not None:
+            _require(token_status, torch.int32, "token_status", device)
+        check("embedding_lookup", load().nntrain_embedding_lookup(
+            device, kind, table.data_ptr(), _ptr(table_scales), block_size, first_value, vocab, width, tokens.data_ptr(),
+            bytes_, count, padding_token, scale, _kind(out), out.data_ptr(), out_stride, _ptr(token_status),
+            _stream_on(device, stream)))
+
+    @staticmethod
+    def gradient(device: int, tokens, out_gradient, table_gradient, scale: float = 1.0, accumulate: bool = False,
+                 padding_token: int = -1, token_status=None, workspace=None, stream=None) -> None:
+        """table_gradient[v] = scale * sum of out_gradient[t] over tokens[t] = v, in
+        the order of t: the whole table, or with `accumulate` added to the rows that
+        are named.  `out_gradient` (tokens, width) fp32 or bf16, any row stride;
+        `table_gradient` (vocab, width) fp32 or bf16, at any place of an arena.
+        `workspace` (optional): uint8 scratch that no call in flight at the same
+        time uses."""
+        count, bytes_ = _tokens(tokens, device)
+        vocab, width, kind = _table(table_gradient, "table_gradient", device, _FLOATS)
+        stride = _rows(out_gradient, "out_gradient", device, width, _FLOATS, count)
+        if token_status is not None:
+            _require(token_status, torch.int32, "token_status", device)
+        workspace, workspace_bytes = _workspace("embedding_gradient", load().nntrain_embedding_gradient_workspace,
+                                                (count, vocab, width), device, workspace, stream)
+        check("embedding_gradient", load().nntrain_embedding_gradient(
+            device, _kind(out_gradient), out_gradient.data_ptr(), stride, tokens.data_ptr(), bytes_, count, padding_token,
+            scale, kind, table_gradient.data_ptr(), vocab, width, int(accumulate), _ptr(token_status), _ptr(workspace),
+            workspace_bytes, _stream_on(device, stream)))
+
+
+def _tokens(tokens: torch.Tensor, device: int) -> tuple[int, int]:
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"tokens must be int32 or int64, got {tokens.dtype}")
+    _require(tokens, tokens.dtype, "tokens", device)
+    return tokens.numel(), tokens.element_size()
+
+
+def _table(table: torch.Tensor, name: str, device: int, dtypes) -> tuple[int, int, int]:
+    """(rows, width, kind) of a token table."""
+    _require(table, table.dtype, name, device)
+    if table.dtype not in dtypes:
+        raise ValueError(f"{name} has type {table.dtype}, expected one of {', '.join(map(str, dtypes))}")
+    if table.dim() != 2 or table.numel() == 0:
+        raise ValueError(f"{name} has shape {tuple(table.shape)}, expected (vocab, width)")
+    return table.shape[0], table.shape[1], 2 if table.dtype == torch.int8 else _kind(table)
