@@ -12,14 +12,18 @@
 // another order every time, so the tokens are sorted (stable) and every row is
 // summed in the order in which its tokens occur, the same bits every time:
 //
-//   sort    one cluster of 8 CTAs: a stable radix sort of (token, position),
-//           9 bits a pass, digit counts exchanged through distributed shared
-//           memory, the cluster's barriers between the passes; no grid-wide wait
-//   rows    a warp takes 32 sorted positions x 256 columns and walks them; a
-//           token that lies inside the 32 is finished, of one that crosses the
-//           border a partial sum goes to scratch.  Further CTAs write the zeros
-//           of the rows no token names (not when adding to what is there)
-//   join    a CTA per crossing token adds its partials in order
+//   sort    pairs (row, position).  Up to 2048 tokens: one CTA, a bitonic sort
+//           in shared memory.  More: one cluster of CTAs, a stable radix sort
+//           of 9 bits a pass, digit counts exchanged through distributed shared
+//           memory, the cluster's barriers between the passes.  (When the whole
+//           table is written, the other SMs write its zeros in the same launch:
+//           they are most of the traffic and take longer than the sort, whose
+//           chain of short waits they hide.)
+//   rows    a warp takes 16 or 32 sorted positions x 128 or 256 columns and walks
+//           them; a token that lies inside them is finished, of one that
+//           crosses the border a partial sum goes to scratch
+//   join    a warp per crossing token adds its partials in order, a CTA where
+//           there are many
 //
 // so a token that is half of the batch is summed by as many warps as its
 // positions are long, and one that occurs once costs one row read and written.
@@ -32,6 +36,8 @@
 #include "nntrain_grad_abi.h"
 
 #include <cooperative_groups.h>
+
+#include <atomic>
 
 namespace ngb {
 namespace {
@@ -68,11 +74,9 @@ struct LookupArguments {
     void* out;
     int* status;
     long long count, out_stride, first_value, block;
-    int width, slices, block_shift;    // block_shift < 0: block is not a power of two; block 0: one scale
+    int width, block_shift;            // block_shift < 0: block is not a power of two; block 0: one scale
     float scale;
 };
-
-constexpr int kLookupGroups = 2;       // groups of 8 values per lane: a warp covers 512 columns
 
 __device__ __forceinline__ float table_scale(const LookupArguments& a, long long value) {
     if (a.block == 0) return __ldg(a.scales);
@@ -80,152 +84,294 @@ __device__ __forceinline__ float table_scale(const LookupArguments& a, long long
     return __ldg(a.scales + (a.block_shift >= 0 ? at >> a.block_shift : at / a.block));
 }
 
-// One warp: one token's row, 512 columns of it.  kVector: 8 neighbouring values
-// per lane and access (of BFP8: in one block); otherwise single values.
-template <int kTable, typename T, bool kVector>
+constexpr int kLookupColumns = 256;    // of a warp: 8 values a lane
+
+template <typename T>
+__device__ __forceinline__ void store_values(T* out, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        store_f4(out, make_float4(v[0], v[1], v[2], v[3]));
+        store_f4(out + 4, make_float4(v[4], v[5], v[6], v[7]));
+    } else {
+        *reinterpret_cast<uint4*>(out) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]),
+                                                    pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    }
+}
+
+// A warp: 256 columns of kTokens neighbouring positions, all their rows in
+// flight together behind one load of the tokens.  kVector: 8 neighbouring
+// values per lane and access (of BFP8: in one block); otherwise single values.
+template <int kTable, typename T, bool kVector, int kTokens>
 __global__ void __launch_bounds__(kThreads)
 embedding_lookup_kernel(LookupArguments a) {
     const int lane = threadIdx.x & 31;
-    const long long task = static_cast<long long>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5);
-    const long long position = task / a.slices;
+    const long long position = (static_cast<long long>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5)) * kTokens;
     if (position >= a.count) return;
-    const int first = static_cast<int>(task - position * a.slices) * (kLookupGroups * 256);
+    const int first = static_cast<int>(blockIdx.y) * kLookupColumns;
+    const int here = static_cast<int>(a.count - position < kTokens ? a.count - position : kTokens);
     bool bad = false;
-    const long long token = a.tokens.at(position, bad);
-    if (bad && a.status != nullptr && lane == 0) atomicExch(a.status, 1);
+    const long long mine = lane < here ? a.tokens.at(position + lane, bad) : -1;
+    if (bad && a.status != nullptr) atomicExch(a.status, 1);
     T* out = static_cast<T*>(a.out) + position * a.out_stride;
-    const long long row = token * a.width;
+    long long token[kTokens];
+    #pragma unroll
+    for (int t = 0; t < kTokens; ++t) token[t] = __shfl_sync(0xffffffffu, mine, t);
     if constexpr (kVector) {
-        float v[kLookupGroups][8] = {};
+        const int column = first + lane * 8;
+        if (column >= a.width) return;
+        constexpr int kWords = kTable == kTableF32 ? 8 : (kTable == kTableBf16 ? 4 : 2);
+        unsigned raw[kTokens][kWords];
+        float row_scale[kTokens];
         #pragma unroll
-        for (int g = 0; g < kLookupGroups; ++g) {
-            const int column = first + (g * 32 + lane) * 8;
-            if (column >= a.width || token < 0) continue;
-            if constexpr (kTable == kTableF32) {
-                const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.table) + row + column);
-                const float4 x = __ldg(p), y = __ldg(p + 1);
-                v[g][0] = x.x; v[g][1] = x.y; v[g][2] = x.z; v[g][3] = x.w;
-                v[g][4] = y.x; v[g][5] = y.y; v[g][6] = y.z; v[g][7] = y.w;
-            } else if constexpr (kTable == kTableBf16) {
-                const uint4 x = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(a.table) + row + column));
-                v[g][0] = bf16_low(x.x); v[g][1] = bf16_high(x.x); v[g][2] = bf16_low(x.y); v[g][3] = bf16_high(x.y);
-                v[g][4] = bf16_low(x.z); v[g][5] = bf16_high(x.z); v[g][6] = bf16_low(x.w); v[g][7] = bf16_high(x.w);
+        for (int t = 0; t < kTokens; ++t) {
+            if (token[t] < 0) continue;
+            const long long at = token[t] * a.width + column;
+            if constexpr (kTable == kTableBfp8) {
+                const uint2 x = __ldg(reinterpret_cast<const uint2*>(static_cast<const signed char*>(a.table) + at));
+                raw[t][0] = x.x; raw[t][1] = x.y;
+                row_scale[t] = table_scale(a, at);
             } else {
-                const uint2 x = __ldg(reinterpret_cast<const uint2*>(static_cast<const signed char*>(a.table) + row + column));
-                const float s = table_scale(a, row + column);
-                const unsigned low = x.x ^ 0x80808080u, high = x.y ^ 0x80808080u;
+                constexpr int kBytes = kTable == kTableF32 ? 4 : 2;
+                const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(a.table) + at * kBytes);
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[g][i] = __fmul_rn(byte_to_float(low, i), s);
-                    v[g][4 + i] = __fmul_rn(byte_to_float(high, i), s);
+                for (int q = 0; q < kWords / 4; ++q) {
+                    const uint4 x = __ldg(p + q);
+                    raw[t][q * 4] = x.x; raw[t][q * 4 + 1] = x.y; raw[t][q * 4 + 2] = x.z; raw[t][q * 4 + 3] = x.w;
                 }
             }
         }
         #pragma unroll
-        for (int g = 0; g < kLookupGroups; ++g) {
-            const int column = first + (g * 32 + lane) * 8;
-            if (column >= a.width) continue;
-            // zeros times an infinite scale would be NaN: a row of no token is not multiplied
+        for (int t = 0; t < kTokens; ++t) {
+            if (t >= here) break;
+            float v[8];
             #pragma unroll
-            for (int i = 0; i < 8; ++i) v[g][i] = token < 0 ? 0.0f : __fmul_rn(v[g][i], a.scale);
-            if constexpr (sizeof(T) == 4) {
-                store_f4(reinterpret_cast<float*>(out) + column, make_float4(v[g][0], v[g][1], v[g][2], v[g][3]));
-                store_f4(reinterpret_cast<float*>(out) + column + 4, make_float4(v[g][4], v[g][5], v[g][6], v[g][7]));
-            } else {
-                *reinterpret_cast<uint4*>(out + column) = make_uint4(pack_bf16(v[g][0], v[g][1]), pack_bf16(v[g][2], v[g][3]),
-                                                                     pack_bf16(v[g][4], v[g][5]), pack_bf16(v[g][6], v[g][7]));
+            for (int i = 0; i < 8; ++i) {
+                if (token[t] < 0) {
+                    v[i] = 0.0f;
+                } else {
+                    if constexpr (kTable == kTableF32) v[i] = __uint_as_float(raw[t][i]);
+                    else if constexpr (kTable == kTableBf16) v[i] = i & 1 ? bf16_high(raw[t][i / 2]) : bf16_low(raw[t][i / 2]);
+                    else v[i] = __fmul_rn(byte_to_float(raw[t][i / 4] ^ 0x80808080u, i & 3), row_scale[t]);
+                    v[i] = __fmul_rn(v[i], a.scale);
+                }
             }
+            store_values(out + t * a.out_stride + column, v);
         }
     } else {
-        #pragma unroll 4
-        for (int i = 0; i < kLookupGroups * 8; ++i) {
-            const int column = first + i * 32 + lane;
-            if (column >= a.width) break;
-            float v = 0.0f;
-            if (token >= 0) {
-                if constexpr (kTable == kTableF32) v = __ldg(static_cast<const float*>(a.table) + row + column);
-                else if constexpr (kTable == kTableBf16) v = bf16_value(__ldg(static_cast<const unsigned short*>(a.table) + row + column));
-                else v = __fmul_rn(static_cast<float>(static_cast<const signed char*>(a.table)[row + column]), table_scale(a, row + column));
-                v = __fmul_rn(v, a.scale);
+        #pragma unroll
+        for (int t = 0; t < kTokens; ++t) {
+            if (t >= here) break;
+            const long long row = token[t] * a.width;
+            #pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int column = first + i * 32 + lane;
+                if (column >= a.width) continue;
+                float v = 0.0f;
+                if (token[t] >= 0) {
+                    if constexpr (kTable == kTableF32) v = __ldg(static_cast<const float*>(a.table) + row + column);
+                    else if constexpr (kTable == kTableBf16) v = bf16_value(__ldg(static_cast<const unsigned short*>(a.table) + row + column));
+                    else v = __fmul_rn(static_cast<float>(__ldg(static_cast<const signed char*>(a.table) + row + column)), table_scale(a, row + column));
+                    v = __fmul_rn(v, a.scale);
+                }
+                if constexpr (sizeof(T) == 4) out[t * a.out_stride + column] = v;
+                else out[t * a.out_stride + column] = bf16_bits(v);
             }
-            if constexpr (sizeof(T) == 4) out[column] = v;
-            else out[column] = bf16_bits(v);
         }
     }
 }
 
 // ---- sort ---------------------------------------------------------------------
 
+constexpr int kSmallSort = 2048;                // tokens that one CTA sorts
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kSortCluster = 8;                 // CTAs (the portable cluster size)
+// CTAs of the sorting cluster: 8 is the portable size.  16, where the device has
+// them, for more tokens than 8 CTAs hold in one load of their warps and nothing
+// beside the sort to hide it (65536 tokens: 35 us with 8, 24 us with 16).
+constexpr int kClusterSmall = 8, kClusterLarge = 16;
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
-constexpr int kSortShared = (kSortWarps * kDigits + 2 * kDigits + 32) * 4;
+constexpr int kSteps = 4;                       // groups of 32 tokens that a warp loads ahead
+constexpr int kSortShared = (kSortWarps + 2) * kDigits * 4;
+constexpr long long kClearBytes = 128 << 10;    // of a CTA beside the sort: 8 stores of a thread; 805 MB at 7.3 TB/s
 
 struct SortArguments {
     Tokens tokens;
-    unsigned* keys[2];                 // passes take turns; the sorted order ends in [0]
-    unsigned* positions[2];
-    unsigned* touched;                 // one bit a row, null when not asked for
-    unsigned* crossing;                // counter of the rows kernel, cleared here
+    uint2* pairs[2];                   // (row, position); passes take turns, the order ends in [0]
+    unsigned* crossing;                // counters of the rows kernel, cleared here
+    unsigned* named;                   // a bit for each row, set where a token names it; null when not asked for
     int* status;
+    char* clear;                       // bytes that the CTAs behind the sort's clear
+    long long clear_bytes;
     unsigned count;
-    int passes, bits;                  // bits of a pass
+    int passes;
 };
 
-// Stable: warps own consecutive stretches of the input, a warp walks its
-// stretch 32 at a time, and equal digits keep the order of their lanes.  Keys
-// are row numbers; positions without a token get the key `vocab`, behind all
-// rows.
+// Zeros to the piece number `piece` of a.clear.  (A table is whole values, so
+// its unaligned ends are whole 2-byte pieces.)
+__device__ void clear_piece(const SortArguments& a, long long piece) {
+    char* begin = a.clear + piece * kClearBytes;
+    const long long left = a.clear_bytes - piece * kClearBytes, bytes = left < kClearBytes ? left : kClearBytes;
+    const int head = static_cast<int>((16u - (reinterpret_cast<std::uintptr_t>(begin) & 15u)) & 15u);
+    const int ends = head < bytes ? head : static_cast<int>(bytes);
+    const int words = static_cast<int>((bytes - ends) / 16);
+    uint4* body = reinterpret_cast<uint4*>(begin + ends);
+    for (int i = threadIdx.x; i < words; i += kSortThreads) body[i] = make_uint4(0, 0, 0, 0);
+    unsigned short* pieces = reinterpret_cast<unsigned short*>(begin);
+    for (int i = threadIdx.x; i < ends / 2; i += kSortThreads) pieces[i] = 0;
+    for (int i = (ends + words * 16) / 2 + threadIdx.x; i < bytes / 2; i += kSortThreads) pieces[i] = 0;
+}
+
+// Ascending sort of `n` (a power of two, 64 at least) numbers in shared memory.
+// Strides up to 32 stay inside the 64 numbers of a warp's pairs, so the CTA
+// waits only around longer ones.
+__device__ void sort_shared(unsigned long long* data, int n) {
+    bool wide = true;
+    for (int k = 2; k <= n; k <<= 1) {
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            if (wide || j > 32) __syncthreads();
+            else __syncwarp();
+            wide = j > 32;
+            const int t = threadIdx.x;
+            if (t < n / 2) {
+                const int i = 2 * t - (t & (j - 1));
+                const unsigned long long x = data[i], y = data[i + j];
+                if ((x > y) == ((i & k) == 0)) {
+                    data[i] = y;
+                    data[i + j] = x;
+                }
+            }
+        }
+    }
+    __syncthreads();
+}
+
+// Up to kSmallSort tokens, `padded` a power of two.  Positions without a token
+// get the row `vocab`, behind all rows.
 __global__ void __launch_bounds__(kSortThreads)
+embedding_small_sort_kernel(SortArguments a, int padded) {
+    __shared__ unsigned long long pairs[kSmallSort];
+    static_assert(kSmallSort == 2 * kSortThreads, "a pair of numbers for each thread");
+    let_next_start();
+    if (blockIdx.x > 0) {
+        clear_piece(a, blockIdx.x - 1);
+        return;
+    }
+    bool bad = false;
+    for (int i = threadIdx.x; i < padded; i += kSortThreads) {
+        const long long token = i < static_cast<int>(a.count) ? a.tokens.at(i, bad) : -1;
+        pairs[i] = (static_cast<unsigned long long>(token < 0 ? a.tokens.vocab : token) << 32) | static_cast<unsigned>(i);
+    }
+    if (threadIdx.x < 2) a.crossing[threadIdx.x] = 0;
+    if (a.named != nullptr)
+        for (long long i = threadIdx.x; i * 32 < a.tokens.vocab; i += kSortThreads) a.named[i] = 0;
+    sort_shared(pairs, padded);                              // (its barriers are behind the zeros)
+    for (int i = threadIdx.x; i < static_cast<int>(a.count); i += kSortThreads) {
+        const unsigned row = static_cast<unsigned>(pairs[i] >> 32);
+        a.pairs[0][i] = make_uint2(row, static_cast<unsigned>(pairs[i]));
+        if (a.named != nullptr && row < a.tokens.vocab) atomicOr(a.named + (row >> 5), 1u << (row & 31u));
+    }
+    if (bad && a.status != nullptr) atomicExch(a.status, 1);
+}
+
+// The first kSteps groups of 32 pairs of a warp's stretch.
+struct Head {
+    uint2 pairs[kSteps];
+};
+
+template <typename Load>
+__device__ __forceinline__ Head load_head(unsigned from, unsigned to, Load load) {
+    Head head;
+    #pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const unsigned at = from + s * 32 + (threadIdx.x & 31);
+        head.pairs[s] = at < to ? load(at) : make_uint2(0, 0);
+    }
+    return head;
+}
+
+// Walks [from, to) 32 at a time, in order: visit(here, pair).  kSteps groups are
+// loaded before the first of them is visited; the first ones are there already.
+template <typename Load, typename Visit>
+__device__ __forceinline__ void walk(unsigned from, unsigned to, Head head, Load load, Visit visit) {
+    const int lane = threadIdx.x & 31;
+    for (unsigned base = from; base < to; base += 32 * kSteps) {
+        if (base != from) head = load_head(base, to, load);
+        #pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+            if (base + s * 32 < to) visit(base + s * 32 + lane < to, head.pairs[s]);
+    }
+}
+
+// Lanes that are here and have the lane's digit: a vote per bit.
+__device__ __forceinline__ unsigned same_digit(bool here, unsigned digit) {
+    unsigned same = __ballot_sync(0xffffffffu, here);
+    #pragma unroll
+    for (int b = 0; b < kDigitBits; ++b) {
+        const bool set = (digit >> b) & 1u;
+        const unsigned votes = __ballot_sync(0xffffffffu, set);
+        same &= set ? votes : ~votes;
+    }
+    return same;
+}
+
+// Stable: warps own consecutive stretches of the input, a warp walks its
+// stretch 32 at a time, and equal digits keep the order of their lanes.  A pair
+// is stored in one piece: the scattered stores of 8 SMs, a 32-byte sector each,
+// are what a pass over many tokens waits for (65536 tokens: 47 us with rows and
+// positions apart, 35 us so).
+//
+// kClear: CTAs behind the first cluster clear; two fit an SM then.
+template <int kCluster, bool kClear>
+__global__ void __launch_bounds__(kSortThreads, kClear ? 2 : 1)
 embedding_sort_kernel(SortArguments a) {
     extern __shared__ unsigned shared[];
     unsigned* counts = shared;                               // [warps][digits]
     unsigned* totals = shared + kSortWarps * kDigits;        // [digits], read by the whole cluster
     unsigned* starts = totals + kDigits;                     // [digits]
-    unsigned* warp_sums = starts + kDigits;                  // [32]
+    __shared__ unsigned sums[32];
+    let_next_start();
+    if (kClear && blockIdx.x >= kCluster) {                  // whole clusters of them: no barrier is shared
+        const long long piece = blockIdx.x - kCluster;
+        if (piece * kClearBytes < a.clear_bytes) clear_piece(a, piece);
+        return;
+    }
     cg::cluster_group cluster = cg::this_cluster();
-    const unsigned rank = cluster.block_rank(), ranks = cluster.num_blocks();
+    const unsigned rank = cluster.block_rank();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const unsigned before = (1u << lane) - 1u;
-    const unsigned workers = ranks * kSortWarps;
-    const unsigned stretch = ((a.count + workers - 1) / workers + 31u) & ~31u;
+    const unsigned below_lane = (1u << lane) - 1u;
+    constexpr unsigned kWorkers = kCluster * kSortWarps;
+    const unsigned stretch = ((a.count + kWorkers - 1) / kWorkers + 31u) & ~31u;
     const unsigned long long begin = static_cast<unsigned long long>(rank * kSortWarps + warp) * stretch;
     const unsigned first = begin < a.count ? static_cast<unsigned>(begin) : a.count;
     const unsigned last = begin + stretch < a.count ? static_cast<unsigned>(begin + stretch) : a.count;
     unsigned* mine = counts + warp * kDigits;
-
-    if (a.touched != nullptr) {
-        const unsigned words = static_cast<unsigned>((a.tokens.vocab + 31) / 32);
-        for (unsigned i = rank * kSortThreads + threadIdx.x; i < words; i += ranks * kSortThreads) a.touched[i] = 0;
+    if (rank == 0 && threadIdx.x < 2) a.crossing[threadIdx.x] = 0;
+    if (kClear && a.named != nullptr) {
+        for (long long i = rank * kSortThreads + threadIdx.x; i * 32 < a.tokens.vocab; i += kCluster * kSortThreads) a.named[i] = 0;
         cluster.sync();
     }
-    if (rank == 0 && threadIdx.x == 0) *a.crossing = 0;
     bool bad = false;
     for (int pass = 0; pass < a.passes; ++pass) {
-        const int out = (a.passes - 1 - pass) & 1, shift = pass * a.bits;
-        const unsigned* in_keys = a.keys[out ^ 1];
-        const unsigned* in_positions = a.positions[out ^ 1];
-        auto key_at = [&](unsigned i) -> unsigned {
-            if (pass > 0) return __ldcg(in_keys + i);
+        const int shift = pass * kDigitBits;
+        uint2* out = (a.passes - 1 - pass) & 1 ? a.pairs[1] : a.pairs[0];
+        const uint2* in = (a.passes - 1 - pass) & 1 ? a.pairs[0] : a.pairs[1];
+        const auto load = [&](unsigned i) {
+            if (pass > 0) return __ldcg(in + i);
             const long long token = a.tokens.at(i, bad);
-            return static_cast<unsigned>(token < 0 ? a.tokens.vocab : token);
+            return make_uint2(static_cast<unsigned>(token < 0 ? a.tokens.vocab : token), i);
         };
-        const unsigned digit_mask = (1u << a.bits) - 1u;
+        const Head head = load_head(first, last, load);
         for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) counts[i] = 0;
         __syncthreads();
-        for (unsigned base = first; base < last; base += 32) {
-            const bool here = base + lane < last;
-            const unsigned key = here ? key_at(base + lane) : 0;
-            const unsigned digit = here ? (key >> shift) & digit_mask : 0xffffffffu;
-            const unsigned same = __match_any_sync(0xffffffffu, digit);
-            if (here && (same & before) == 0) mine[digit] += __popc(same);
-            if (pass == 0 && here && a.touched != nullptr && key < static_cast<unsigned long long>(a.tokens.vocab))
-                atomicOr(a.touched + (key >> 5), 1u << (key & 31u));
+        walk(first, last, head, load, [&](bool here, uint2 pair) {
+            const unsigned digit = (pair.x >> shift) & (kDigits - 1), same = same_digit(here, digit);
+            if (here && (same & below_lane) == 0) mine[digit] += __popc(same);
+            if (kClear && pass == 0 && here && a.named != nullptr && pair.x < a.tokens.vocab)
+                atomicOr(a.named + (pair.x >> 5), 1u << (pair.x & 31u));
             __syncwarp();
-        }
+        });
         __syncthreads();
         if (threadIdx.x < kDigits) {
             unsigned sum = 0;
+            #pragma unroll 8
             for (int w = 0; w < kSortWarps; ++w) {
                 const unsigned n = counts[w * kDigits + threadIdx.x];
                 counts[w * kDigits + threadIdx.x] = sum;
@@ -237,7 +383,8 @@ embedding_sort_kernel(SortArguments a) {
         // first place of this CTA's share of each digit
         unsigned below = 0, all = 0, inclusive = 0;
         if (threadIdx.x < kDigits) {
-            for (unsigned r = 0; r < ranks; ++r) {
+            #pragma unroll
+            for (unsigned r = 0; r < kCluster; ++r) {
                 const unsigned n = *cluster.map_shared_rank(totals + threadIdx.x, r);
                 below += r < rank ? n : 0;
                 all += n;
@@ -248,62 +395,61 @@ embedding_sort_kernel(SortArguments a) {
                 const unsigned n = __shfl_up_sync(0xffffffffu, inclusive, offset);
                 inclusive += lane >= offset ? n : 0;
             }
-            if (lane == 31) warp_sums[warp] = inclusive;
+            if (lane == 31) sums[warp] = inclusive;
         }
         __syncthreads();
         if (threadIdx.x < kDigits) {
-            for (int w = 0; w < warp; ++w) inclusive += warp_sums[w];
+            for (int w = 0; w < warp; ++w) inclusive += sums[w];
             starts[threadIdx.x] = inclusive - all + below;
         }
         __syncthreads();
-        for (unsigned base = first; base < last; base += 32) {
-            const bool here = base + lane < last;
-            const unsigned key = here ? key_at(base + lane) : 0;
-            const unsigned position = !here ? 0 : (pass > 0 ? __ldcg(in_positions + base + lane) : base + lane);
-            const unsigned digit = here ? (key >> shift) & digit_mask : 0xffffffffu;
-            const unsigned same = __match_any_sync(0xffffffffu, digit);
-            if (here) {
-                const unsigned place = starts[digit] + mine[digit] + __popc(same & before);
-                if (place < a.count) {           // always, unless the tokens change while they are sorted
-                    a.keys[out][place] = key;
-                    a.positions[out][place] = position;
-                }
-            }
+        walk(first, last, head, load, [&](bool here, uint2 pair) {
+            const unsigned digit = (pair.x >> shift) & (kDigits - 1), same = same_digit(here, digit);
+            const unsigned before = same & below_lane;
+            const unsigned place = here ? starts[digit] + mine[digit] + __popc(before) : a.count;
+            if (place < a.count) out[place] = pair;          // (it is, unless the tokens change while they are sorted)
             __syncwarp();
-            if (here && (same & before) == 0) mine[digit] += __popc(same);
+            if (here && before == 0) mine[digit] += __popc(same);
             __syncwarp();
-        }
-        cluster.sync();
+        });
+        cluster.sync();                                      // the pass is in memory, and nobody reads these totals
     }
     if (bad && a.status != nullptr) atomicExch(a.status, 1);
 }
 
 // ---- rows and join --------------------------------------------------------------
 
-constexpr int kChunkPositions = 32;             // sorted positions of a warp
-constexpr int kSliceColumns = 256;              // columns of a warp: 8 a lane
-constexpr int kZeroRows = 32;                   // rows of a CTA that writes zeros: one word of the bitmap
+// Sorted positions of a warp.  32, so that few tokens cross; 16 where that
+// leaves the SMs less than 16 warps each.
+constexpr int kChunkMost = 32, kChunkLeast = 16;
+constexpr int kZeroRows = 32;                   // rows of a CTA that writes late zeros: one word of the bitmap
+// Columns of a warp: one 128-bit load of a lane, or 8 single values.
+template <typename G, bool kVector>
+__host__ __device__ constexpr int lane_values() { return kVector && sizeof(G) == 4 ? 4 : 8; }
 
 struct RowsArguments {
-    const unsigned* keys;
-    const unsigned* positions;
-    const unsigned* touched;
-    unsigned* crossing;                // [0] count, then the chunks in which a crossing token begins
+    const uint2* pairs;                // sorted (row, position)
+    unsigned* crossing;                // tokens that cross chunks: number of short and of long ones, then
+    unsigned* crossing_short;          // the chunks in which they begin
+    unsigned* crossing_long;
     float* tails;                      // [chunk][width]: sum up to the chunk's end of a token that goes on
     float* heads;                      // [chunk][width]: rest of a token that began in an earlier chunk
     const void* gradient;              // dout
     void* table;
     long long gradient_stride;
-    unsigned count, vocab, chunks;
-    int width, slices, row_ctas;
+    const unsigned* named;             // the sort's bitmap
+    long long late;                    // rows from here on were not cleared beside the sort
+    unsigned count, vocab, chunk, chunks;    // chunk: positions of one
+    int width, slices, row_ctas, long_ctas, join_ctas;
+    unsigned late_groups, join_groups; // groups of kZeroRows rows from `late` on, and the first of the join's
     float scale;
     bool accumulate;
 };
 
-// Column of the lane's i-th value: 8 neighbours, or every 32nd.
-template <bool kVector>
+// Column of the lane's i-th value: neighbours, or every 32nd.
+template <int kValues, bool kVector>
 __device__ __forceinline__ int lane_column(int first, int lane, int i) {
-    return kVector ? first + lane * 8 + i : first + i * 32 + lane;
+    return kVector ? first + lane * kValues + i : first + i * 32 + lane;
 }
 
 template <typename T>
@@ -313,41 +459,34 @@ __device__ __forceinline__ float value_of(T raw) {
 }
 
 // table[row] = scale * sum (+ what is there), rounded once.
-template <typename T, bool kVector>
-__device__ __forceinline__ void store_row(const RowsArguments& a, unsigned row, int first, int lane, const float (&sum)[8]) {
+template <typename T, int kValues, bool kVector>
+__device__ __forceinline__ void store_row(const RowsArguments& a, unsigned row, int first, int lane, const float (&sum)[kValues]) {
     T* out = static_cast<T*>(a.table) + static_cast<long long>(row) * a.width;
-    float v[8];
     if constexpr (kVector) {
-        const int column = lane_column<true>(first, lane, 0);
+        const int column = lane_column<kValues, true>(first, lane, 0);
         if (column >= a.width) return;
         out += column;
         #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(sum[i], a.scale);
-        if constexpr (sizeof(T) == 4) {
+        for (int q = 0; q < kValues; q += 4) {
+            float x[4] = {};
             if (a.accumulate) {
-                const float4 x = load_f4(out), y = load_f4(out + 4);
-                v[0] = __fmaf_rn(sum[0], a.scale, x.x); v[1] = __fmaf_rn(sum[1], a.scale, x.y);
-                v[2] = __fmaf_rn(sum[2], a.scale, x.z); v[3] = __fmaf_rn(sum[3], a.scale, x.w);
-                v[4] = __fmaf_rn(sum[4], a.scale, y.x); v[5] = __fmaf_rn(sum[5], a.scale, y.y);
-                v[6] = __fmaf_rn(sum[6], a.scale, y.z); v[7] = __fmaf_rn(sum[7], a.scale, y.w);
+                if constexpr (sizeof(T) == 4) {
+                    const float4 old = load_f4(out + q);
+                    x[0] = old.x; x[1] = old.y; x[2] = old.z; x[3] = old.w;
+                } else {
+                    const uint2 old = *reinterpret_cast<const uint2*>(out + q);
+                    x[0] = bf16_low(old.x); x[1] = bf16_high(old.x); x[2] = bf16_low(old.y); x[3] = bf16_high(old.y);
+                }
             }
-            store_f4(out, make_float4(v[0], v[1], v[2], v[3]));
-            store_f4(out + 4, make_float4(v[4], v[5], v[6], v[7]));
-        } else {
-            if (a.accumulate) {
-                const uint4 x = *reinterpret_cast<const uint4*>(out);
-                v[0] = __fmaf_rn(sum[0], a.scale, bf16_low(x.x)); v[1] = __fmaf_rn(sum[1], a.scale, bf16_high(x.x));
-                v[2] = __fmaf_rn(sum[2], a.scale, bf16_low(x.y)); v[3] = __fmaf_rn(sum[3], a.scale, bf16_high(x.y));
-                v[4] = __fmaf_rn(sum[4], a.scale, bf16_low(x.z)); v[5] = __fmaf_rn(sum[5], a.scale, bf16_high(x.z));
-                v[6] = __fmaf_rn(sum[6], a.scale, bf16_low(x.w)); v[7] = __fmaf_rn(sum[7], a.scale, bf16_high(x.w));
-            }
-            *reinterpret_cast<uint4*>(out) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]),
-                                                        pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = a.accumulate ? __fmaf_rn(sum[q + i], a.scale, x[i]) : __fmul_rn(sum[q + i], a.scale);
+            if constexpr (sizeof(T) == 4) store_f4(out + q, make_float4(x[0], x[1], x[2], x[3]));
+            else *reinterpret_cast<uint2*>(out + q) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
         }
     } else {
         #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int column = lane_column<false>(first, lane, i);
+        for (int i = 0; i < kValues; ++i) {
+            const int column = lane_column<kValues, false>(first, lane, i);
             if (column >= a.width) continue;
             const float x = a.accumulate ? __fmaf_rn(sum[i], a.scale, value_of(out[column])) : __fmul_rn(sum[i], a.scale);
             if constexpr (sizeof(T) == 4) out[column] = x;
@@ -356,31 +495,26 @@ __device__ __forceinline__ void store_row(const RowsArguments& a, unsigned row, 
     }
 }
 
-template <bool kVector>
-__device__ __forceinline__ void store_partial(float* partials, unsigned chunk, int width, int first, int lane, const float (&sum)[8]) {
+template <int kValues, bool kVector>
+__device__ __forceinline__ void store_partial(float* partials, unsigned chunk, int width, int first, int lane,
+                                              const float (&sum)[kValues]) {
     float* out = partials + static_cast<long long>(chunk) * width;
-    if constexpr (kVector) {
-        const int column = lane_column<true>(first, lane, 0);
-        if (column >= width) return;
-        store_f4(out + column, make_float4(sum[0], sum[1], sum[2], sum[3]));
-        store_f4(out + column + 4, make_float4(sum[4], sum[5], sum[6], sum[7]));
-    } else {
-        #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int column = lane_column<false>(first, lane, i);
-            if (column < width) out[column] = sum[i];
-        }
+    #pragma unroll
+    for (int i = 0; i < kValues; i += kVector ? 4 : 1) {
+        const int column = lane_column<kValues, kVector>(first, lane, i);
+        if (column >= width) continue;
+        if constexpr (kVector) store_f4(out + column, make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]));
+        else out[column] = sum[i];
     }
 }
 
-// The zeros of 32 rows, those that the bitmap does not name.
+// The zeros of 32 rows, those that no token names.
 template <typename T>
 __device__ void zero_rows(const RowsArguments& a, unsigned group) {
-    const unsigned touched = a.touched[group];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int r = warp; r < kZeroRows; r += kWarpsPerCta) {
-        const long long row = static_cast<long long>(group) * kZeroRows + r;
-        if (row >= a.vocab || ((touched >> r) & 1u)) continue;
+        const long long row = a.late + static_cast<long long>(group) * kZeroRows + r;
+        if (row >= a.vocab || ((a.named[row >> 5] >> (row & 31)) & 1u)) continue;
         T* out = static_cast<T*>(a.table) + row * a.width;
         constexpr int kPerWord = 16 / sizeof(T);
         int head = static_cast<int>((16u - (reinterpret_cast<std::uintptr_t>(out) & 15u)) & 15u) / static_cast<int>(sizeof(T));
@@ -392,47 +526,50 @@ __device__ void zero_rows(const RowsArguments& a, unsigned group) {
     }
 }
 
+// A token that goes on for this many chunks is long: a CTA adds its partials,
+// not a warp.
+constexpr unsigned kLongChunks = 16;
+
 template <typename G, typename T, bool kVector>
 __global__ void __launch_bounds__(kThreads)
 embedding_rows_kernel(RowsArguments a) {
+    constexpr int kValues = lane_values<G, kVector>();
+    const int lane = threadIdx.x & 31;
+    const unsigned task = blockIdx.x * kWarpsPerCta + (threadIdx.x >> 5);
+    const unsigned chunk = task / a.slices, size = a.chunk, base = chunk * size;
     wait_for_previous();
     let_next_start();
     if (static_cast<int>(blockIdx.x) >= a.row_ctas) {
         zero_rows<T>(a, blockIdx.x - a.row_ctas);
         return;
     }
-    const int lane = threadIdx.x & 31;
-    const unsigned task = blockIdx.x * kWarpsPerCta + (threadIdx.x >> 5);
-    const unsigned chunk = task / a.slices;
     if (chunk >= a.chunks) return;
-    const int first = static_cast<int>(task - chunk * a.slices) * kSliceColumns;
-    const unsigned base = chunk * kChunkPositions;
-    const unsigned key = base + lane < a.count ? a.keys[base + lane] : a.vocab;
-    const unsigned position = base + lane < a.count ? a.positions[base + lane] : 0;
-    const unsigned key_before = chunk > 0 ? a.keys[base - 1] : a.vocab;
-    const unsigned key_behind = base + kChunkPositions < a.count ? a.keys[base + kChunkPositions] : a.vocab;
+    const int first = static_cast<int>(task - chunk * a.slices) * (kValues * 32);
+    const uint2 none = make_uint2(a.vocab, 0);
+    const uint2 pair = lane < static_cast<int>(size) && base + lane < a.count ? a.pairs[base + lane] : none;
+    const unsigned key = pair.x, position = pair.y;
+    const unsigned key_before = chunk > 0 ? a.pairs[base - 1].x : a.vocab;
+    const unsigned key_behind = base + size < a.count ? a.pairs[base + size].x : a.vocab;
     const int n = __popc(__ballot_sync(0xffffffffu, key != a.vocab));    // rows come first
-    constexpr int kBatch = sizeof(G) == 4 ? 4 : 8;                          // rows whose loads are in flight together
+    constexpr int kBatch = kVector ? 8 : 4;          // rows whose loads are in flight together
     const G* gradient = static_cast<const G*>(a.gradient);
-    float sum[8] = {};
+    float sum[kValues] = {};
     bool begun_here = __shfl_sync(0xffffffffu, key, 0) != key_before;
     for (int j = 0; j < n; j += kBatch) {
-        uint4 raw[kBatch][sizeof(G) / 2];
-        G single[kBatch][8];
+        uint4 raw[kBatch];
+        G single[kBatch][kValues];
         #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             const unsigned at = __shfl_sync(0xffffffffu, position, (j + b) & 31);
             if (j + b >= n) continue;
             const G* row = gradient + static_cast<long long>(at) * a.gradient_stride;
             if constexpr (kVector) {
-                const int column = lane_column<true>(first, lane, 0);
-                #pragma unroll
-                for (int h = 0; h < static_cast<int>(sizeof(G)) / 2; ++h)
-                    raw[b][h] = column < a.width ? __ldcs(reinterpret_cast<const uint4*>(row + column) + h) : make_uint4(0, 0, 0, 0);
+                const int column = lane_column<kValues, true>(first, lane, 0);
+                raw[b] = column < a.width ? __ldcs(reinterpret_cast<const uint4*>(row + column)) : make_uint4(0, 0, 0, 0);
             } else {
                 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int column = lane_column<false>(first, lane, i);
+                for (int i = 0; i < kValues; ++i) {
+                    const int column = lane_column<kValues, false>(first, lane, i);
                     single[b][i] = column < a.width ? __ldcs(row + column) : G(0);
                 }
             }
@@ -441,40 +578,38 @@ embedding_rows_kernel(RowsArguments a) {
         for (int b = 0; b < kBatch; ++b) {
             if (j + b >= n) continue;
             const unsigned here = __shfl_sync(0xffffffffu, key, j + b);
-            const unsigned next = j + b + 1 < kChunkPositions ? __shfl_sync(0xffffffffu, key, (j + b + 1) & 31) : key_behind;
+            const unsigned next = j + b + 1 < static_cast<int>(size) ? __shfl_sync(0xffffffffu, key, (j + b + 1) & 31) : key_behind;
             if constexpr (kVector) {
-                if constexpr (sizeof(G) == 4) {
-                    const uint4 x = raw[b][0], y = raw[b][1];
-                    const float v[8] = {__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w),
-                                        __uint_as_float(y.x), __uint_as_float(y.y), __uint_as_float(y.z), __uint_as_float(y.w)};
-                    #pragma unroll
-                    for (int i = 0; i < 8; ++i) sum[i] = __fadd_rn(sum[i], v[i]);
-                } else {
-                    const uint4 x = raw[b][0];
-                    const unsigned w[4] = {x.x, x.y, x.z, x.w};
-                    #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                const unsigned w[4] = {raw[b].x, raw[b].y, raw[b].z, raw[b].w};
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (sizeof(G) == 4) {
+                        sum[i] = __fadd_rn(sum[i], __uint_as_float(w[i]));
+                    } else {
                         sum[2 * i] = __fadd_rn(sum[2 * i], bf16_low(w[i]));
                         sum[2 * i + 1] = __fadd_rn(sum[2 * i + 1], bf16_high(w[i]));
                     }
                 }
             } else {
                 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum[i] = __fadd_rn(sum[i], value_of(single[b][i]));
+                for (int i = 0; i < kValues; ++i) sum[i] = __fadd_rn(sum[i], value_of(single[b][i]));
             }
-            if (next == here && j + b + 1 < kChunkPositions) continue;      // the token goes on in this chunk
-            const bool goes_on = next == here;
-            if (goes_on) {
-                store_partial<kVector>(a.tails, chunk, a.width, first, lane, sum);
-                if (begun_here && first == 0 && lane == 0) a.crossing[1 + atomicAdd(a.crossing, 1u)] = chunk;
+            if (next == here && j + b + 1 < static_cast<int>(size)) continue;      // the token goes on in this chunk
+            if (next == here) {
+                store_partial<kValues, kVector>(a.tails, chunk, a.width, first, lane, sum);
+                if (begun_here && first == 0 && lane == 0) {
+                    const unsigned long long far = static_cast<unsigned long long>(chunk + kLongChunks) * size;
+                    const bool is_long = far < a.count && a.pairs[far].x == here;
+                    (is_long ? a.crossing_long : a.crossing_short)[atomicAdd(a.crossing + is_long, 1u)] = chunk;
+                }
             } else if (!begun_here) {
-                store_partial<kVector>(a.heads, chunk, a.width, first, lane, sum);
+                store_partial<kValues, kVector>(a.heads, chunk, a.width, first, lane, sum);
             } else {
-                store_row<T, kVector>(a, here, first, lane, sum);
+                store_row<T, kValues, kVector>(a, here, first, lane, sum);
             }
             begun_here = true;
             #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
+            for (int i = 0; i < kValues; ++i) sum[i] = 0.0f;
         }
     }
 }
@@ -487,7 +622,7 @@ __device__ unsigned last_chunk_of(const RowsArguments& a, unsigned key, unsigned
     unsigned step = 1;
     while (high - low > 1) {
         const unsigned long long probe = low + static_cast<unsigned long long>(step) * (lane + 1);
-        const bool holds = probe < high && a.keys[probe * kChunkPositions] == key;
+        const bool holds = probe < high && a.pairs[probe * a.chunk].x == key;
         const unsigned held = __popc(__ballot_sync(0xffffffffu, holds));   // the first `held` probes hold it
         const unsigned long long beyond = low + static_cast<unsigned long long>(step) * (held + 1);
         low += step * held;
@@ -497,53 +632,69 @@ __device__ unsigned last_chunk_of(const RowsArguments& a, unsigned key, unsigned
     return low;
 }
 
-// A CTA per token that crosses chunks (and 256 columns): tails[begin], the
-// tails of the chunks between, heads[end]; each of 8 warps adds an eighth of
-// them in order, the eighths are added in order.
-template <typename T, bool kVector>
-__global__ void __launch_bounds__(kThreads)
-embedding_join_kernel(RowsArguments a) {
-    __shared__ float sums[kWarpsPerCta][kSliceColumns];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    wait_for_previous();
-    const unsigned tasks = a.crossing[0] * a.slices;
-    for (unsigned task = blockIdx.x; task < tasks; task += gridDim.x) {
-        const unsigned begin = a.crossing[1 + task / a.slices];
-        const int first = static_cast<int>(task % a.slices) * kSliceColumns;
-        const unsigned key = a.keys[begin * kChunkPositions + kChunkPositions - 1];
-        const unsigned end = last_chunk_of(a, key, begin, lane);
-        const unsigned parts = end - begin + 1, share = (parts + kWarpsPerCta - 1) / kWarpsPerCta;
-        const unsigned from = warp * share, to = from + share < parts ? from + share : parts;
-        float sum[8] = {};
-        #pragma unroll 4
-        for (unsigned p = from; p < to; ++p) {
-            const float* partial = (begin + p == end ? a.heads : a.tails) + static_cast<long long>(begin + p) * a.width;
+// sum += the partials [from, to) of the token that begins in chunk `begin`: the
+// tails of its chunks, the head of the last one.
+template <int kValues, bool kVector>
+__device__ __forceinline__ void add_partials(const RowsArguments& a, unsigned begin, unsigned end, unsigned from, unsigned to,
+                                             int first, int lane, float (&sum)[kValues]) {
+    #pragma unroll 4
+    for (unsigned p = from; p < to; ++p) {
+        const float* partial = (begin + p == end ? a.heads : a.tails) + static_cast<long long>(begin + p) * a.width;
+        #pragma unroll
+        for (int i = 0; i < kValues; i += kVector ? 4 : 1) {
+            const int column = lane_column<kValues, kVector>(first, lane, i);
+            if (column >= a.width) continue;
             if constexpr (kVector) {
-                const int column = lane_column<true>(first, lane, 0);
-                if (column < a.width) {
-                    const float4 x = load_f4(partial + column), y = load_f4(partial + column + 4);
-                    sum[0] = __fadd_rn(sum[0], x.x); sum[1] = __fadd_rn(sum[1], x.y);
-                    sum[2] = __fadd_rn(sum[2], x.z); sum[3] = __fadd_rn(sum[3], x.w);
-                    sum[4] = __fadd_rn(sum[4], y.x); sum[5] = __fadd_rn(sum[5], y.y);
-                    sum[6] = __fadd_rn(sum[6], y.z); sum[7] = __fadd_rn(sum[7], y.w);
-                }
+                const float4 x = load_f4(partial + column);
+                sum[i] = __fadd_rn(sum[i], x.x); sum[i + 1] = __fadd_rn(sum[i + 1], x.y);
+                sum[i + 2] = __fadd_rn(sum[i + 2], x.z); sum[i + 3] = __fadd_rn(sum[i + 3], x.w);
             } else {
-                #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int column = lane_column<false>(first, lane, i);
-                    if (column < a.width) sum[i] = __fadd_rn(sum[i], partial[column]);
-                }
+                sum[i] = __fadd_rn(sum[i], partial[column]);
             }
         }
+    }
+}
+
+// The first CTAs take the long crossing tokens (and a slice of their columns):
+// each of 8 warps adds an eighth of the partials in order, the eighths are
+// added in order.  In the others a warp takes a short one.
+template <typename T, int kValues, bool kVector>
+__global__ void __launch_bounds__(kThreads)
+embedding_join_kernel(RowsArguments a) {
+    __shared__ float sums[kWarpsPerCta][kValues * 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool is_long = static_cast<int>(blockIdx.x) < a.long_ctas;
+    wait_for_previous();
+    if (static_cast<int>(blockIdx.x) >= a.join_ctas) {
+        zero_rows<T>(a, a.join_groups + blockIdx.x - a.join_ctas);
+        return;
+    }
+    const unsigned long long tasks = static_cast<unsigned long long>(a.crossing[is_long]) * a.slices;
+    const unsigned long long step = is_long ? a.long_ctas : static_cast<unsigned long long>(a.join_ctas - a.long_ctas) * kWarpsPerCta;
+    unsigned long long task = is_long ? blockIdx.x : static_cast<unsigned long long>(blockIdx.x - a.long_ctas) * kWarpsPerCta + warp;
+    for (; task < tasks; task += step) {
+        const unsigned begin = (is_long ? a.crossing_long : a.crossing_short)[task / a.slices];
+        const int first = static_cast<int>(task % a.slices) * (kValues * 32);
+        const unsigned key = a.pairs[begin * a.chunk + a.chunk - 1].x;
+        const unsigned end = last_chunk_of(a, key, begin, lane), parts = end - begin + 1;
+        float sum[kValues] = {};
+        if (!is_long) {
+            add_partials<kValues, kVector>(a, begin, end, 0, parts, first, lane, sum);
+            store_row<T, kValues, kVector>(a, key, first, lane, sum);
+            continue;
+        }
+        const unsigned share = (parts + kWarpsPerCta - 1) / kWarpsPerCta;
+        const unsigned from = warp * share < parts ? warp * share : parts, to = from + share < parts ? from + share : parts;
+        add_partials<kValues, kVector>(a, begin, end, from, to, first, lane, sum);
         #pragma unroll
-        for (int i = 0; i < 8; ++i) sums[warp][i * 32 + lane] = sum[i];
+        for (int i = 0; i < kValues; ++i) sums[warp][i * 32 + lane] = sum[i];
         __syncthreads();
         if (warp == 0) {
             for (int w = 1; w < kWarpsPerCta; ++w) {
                 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum[i] = __fadd_rn(sum[i], sums[w][i * 32 + lane]);
+                for (int i = 0; i < kValues; ++i) sum[i] = __fadd_rn(sum[i], sums[w][i * 32 + lane]);
             }
-            store_row<T, kVector>(a, key, first, lane, sum);
+            store_row<T, kValues, kVector>(a, key, first, lane, sum);
         }
         __syncthreads();
     }
@@ -551,18 +702,30 @@ embedding_join_kernel(RowsArguments a) {
 
 // ---- entry points ----------------------------------------------------------------
 
+constexpr long long kLateBytes = 128ll << 20;
 constexpr long long kMostTokens = (1ll << 31) - 64, kMostVocab = 1ll << 31;
-constexpr int kMostWidth = 1 << 24;
+constexpr int kMostWidth = (1 << 24) - 256;     // 65535 slices of the lookup
 
 bool valid_sizes(long long count, long long vocab, int width) {
     return count >= 0 && count <= kMostTokens && vocab >= 1 && vocab <= kMostVocab && width >= 1 && width <= kMostWidth;
 }
 
-template <int kTable, typename T>
-cudaError_t run_lookup(const LookupArguments& a, bool vector_ok, int grid, cudaStream_t stream) {
-    if (vector_ok) embedding_lookup_kernel<kTable, T, true><<<grid, kThreads, 0, stream>>>(a);
-    else embedding_lookup_kernel<kTable, T, false><<<grid, kThreads, 0, stream>>>(a);
+template <int kTable, typename T, int kTokens>
+cudaError_t launch_lookup(const LookupArguments& a, bool vector_ok, cudaStream_t stream) {
+    constexpr int kCtaTokens = kWarpsPerCta * kTokens;
+    const dim3 grid(static_cast<unsigned>((a.count + kCtaTokens - 1) / kCtaTokens),
+                    static_cast<unsigned>((a.width + kLookupColumns - 1) / kLookupColumns));
+    if (vector_ok) embedding_lookup_kernel<kTable, T, true, kTokens><<<grid, kThreads, 0, stream>>>(a);
+    else embedding_lookup_kernel<kTable, T, false, kTokens><<<grid, kThreads, 0, stream>>>(a);
     return cudaPeekAtLastError();
+}
+
+// Four tokens a warp once that still leaves each SM 16 warps, else one.
+template <int kTable, typename T>
+cudaError_t run_lookup(const LookupArguments& a, bool vector_ok, cudaStream_t stream) {
+    const long long warps = a.count * ((a.width + kLookupColumns - 1) / kLookupColumns);
+    return warps >= 64ll * sm_count() ? launch_lookup<kTable, T, 4>(a, vector_ok, stream)
+                                      : launch_lookup<kTable, T, 1>(a, vector_ok, stream);
 }
 
 int lookup(int device, int table_kind, const void* table, const float* scales, int block_size, long long first_value,
@@ -577,34 +740,30 @@ int lookup(int device, int table_kind, const void* table, const float* scales, i
         !aligned_for(scales, 4) || !aligned_for(token_status, 4))
         return static_cast<int>(cudaErrorInvalidValue);
     if (count == 0) return static_cast<int>(cudaSuccess);
-    constexpr int kColumns = kLookupGroups * 256;
-    const int slices = (width + kColumns - 1) / kColumns;
-    const long long ctas = (count * slices + kWarpsPerCta - 1) / kWarpsPerCta;
-    if (ctas > 2147483647ll) return static_cast<int>(cudaErrorInvalidValue);
     const DeviceScope scope(device);
     if (scope.status() != cudaSuccess) return scope.status();
     int shift = -1;
     if (block_size > 0 && (block_size & (block_size - 1)) == 0)
         for (shift = 0; (1 << shift) < block_size;) ++shift;
     const LookupArguments a{Tokens{tokens, token_bytes, padding_token, vocab}, table, scales, out, token_status, count,
-                            out_stride, first_value, block_size, width, slices, shift, scale};
+                            out_stride, first_value, block_size, width, shift, scale};
     const bool vector_ok = width % 8 == 0 && aligned_for(table, table_kind == kTableBfp8 ? 8 : 16) && aligned_for(out, 16) &&
                            out_stride * out_bytes % 16 == 0 &&
                            (table_kind != kTableBfp8 || block_size == 0 || (block_size % 8 == 0 && first_value % 8 == 0));
-    const int grid = static_cast<int>(ctas);
     if (out_kind == 0) {
-        if (table_kind == kTableF32) return static_cast<int>(run_lookup<kTableF32, float>(a, vector_ok, grid, stream));
-        if (table_kind == kTableBf16) return static_cast<int>(run_lookup<kTableBf16, float>(a, vector_ok, grid, stream));
-        return static_cast<int>(run_lookup<kTableBfp8, float>(a, vector_ok, grid, stream));
+        if (table_kind == kTableF32) return static_cast<int>(run_lookup<kTableF32, float>(a, vector_ok, stream));
+        if (table_kind == kTableBf16) return static_cast<int>(run_lookup<kTableBf16, float>(a, vector_ok, stream));
+        return static_cast<int>(run_lookup<kTableBfp8, float>(a, vector_ok, stream));
     }
-    if (table_kind == kTableF32) return static_cast<int>(run_lookup<kTableF32, unsigned short>(a, vector_ok, grid, stream));
-    if (table_kind == kTableBf16) return static_cast<int>(run_lookup<kTableBf16, unsigned short>(a, vector_ok, grid, stream));
-    return static_cast<int>(run_lookup<kTableBfp8, unsigned short>(a, vector_ok, grid, stream));
+    if (table_kind == kTableF32) return static_cast<int>(run_lookup<kTableF32, unsigned short>(a, vector_ok, stream));
+    if (table_kind == kTableBf16) return static_cast<int>(run_lookup<kTableBf16, unsigned short>(a, vector_ok, stream));
+    return static_cast<int>(run_lookup<kTableBfp8, unsigned short>(a, vector_ok, stream));
 }
 
 // Scratch of one gradient call, every part on a 256-byte boundary.
 struct GradientScratch {
-    long long keys[2], positions[2], touched, crossing, tails, heads, bytes;
+    long long pairs[2], named, crossing, crossing_short, crossing_long, tails, heads, bytes;
+    int chunk;
     long long chunks;
 };
 
@@ -615,44 +774,110 @@ GradientScratch gradient_scratch(long long count, long long vocab, int width) {
         s.bytes += (bytes + 255) / 256 * 256;
         return at;
     };
-    s.chunks = (count + kChunkPositions - 1) / kChunkPositions;
-    for (int i = 0; i < 2; ++i) {
-        s.keys[i] = take(count * 4);
-        s.positions[i] = take(count * 4);
-    }
-    s.touched = take((vocab + 31) / 32 * 4);
-    s.crossing = take((s.chunks + 1) * 4);
+    // (256 columns a warp; with 148 SMs this is 16 warps each)
+    const long long warps = (count + kChunkMost - 1) / kChunkMost * ((width + 255) / 256);
+    s.chunk = warps < 148 * 16 ? kChunkLeast : kChunkMost;
+    s.chunks = (count + s.chunk - 1) / s.chunk;
+    for (int i = 0; i < 2; ++i) s.pairs[i] = take(count * 8);
+    s.named = take((vocab + 31) / 32 * 4);
+    s.crossing = take(8);
+    s.crossing_short = take(s.chunks * 4);
+    s.crossing_long = take((s.chunks / kLongChunks + 1) * 4);
     s.tails = take(s.chunks * width * 4);
     s.heads = take(s.chunks * width * 4);
     return s;
 }
 
-cudaError_t launch_sort(const SortArguments& a, cudaStream_t stream) {
-    // a dynamic-shared-memory limit belongs to the device's context; setting it costs a fraction of the launch
-    cudaError_t e = cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortShared);
-    if (e != cudaSuccess) return e;
-    cudaLaunchAttribute attribute{};
+using SortKernel = void (*)(SortArguments);
+
+cudaLaunchConfig_t cluster_launch(int cluster, long long ctas, cudaLaunchAttribute& attribute, cudaStream_t stream) {
     attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = kSortCluster;
+    attribute.val.clusterDim.x = cluster;
     attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(kSortCluster);
+    config.gridDim = dim3(static_cast<unsigned>(ctas));
     config.blockDim = dim3(kSortThreads);
     config.dynamicSmemBytes = kSortShared;
     config.stream = stream;
     config.attrs = &attribute;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, embedding_sort_kernel, a);
+    return config;
+}
+
+template <int kCluster>
+cudaError_t launch_cluster(SortKernel kernel, long long ctas, const SortArguments& a, cudaStream_t stream) {
+    // the limit belongs to the device's context; setting it costs a fraction of a launch
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortShared);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute attribute{};
+    const cudaLaunchConfig_t config = cluster_launch(kCluster, ctas, attribute, stream);
+    return cudaLaunchKernelEx(&config, kernel, a);
+}
+
+// Whether the current device runs clusters of 16 such CTAs: asked once per
+// device, after which the kernel may be launched so.
+bool large_clusters() {
+    constexpr int kDevices = 64;
+    static std::atomic<int> known[kDevices];     // 0: not asked yet, 1: no, 2: yes
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kDevices) return false;
+    int answer = known[device].load(std::memory_order_relaxed);
+    if (answer == 0) {
+        SortKernel kernel = embedding_sort_kernel<kClusterLarge, false>;
+        cudaLaunchAttribute attribute{};
+        const cudaLaunchConfig_t config = cluster_launch(kClusterLarge, kClusterLarge, attribute, nullptr);
+        int clusters = 0;
+        const bool can = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortShared) == cudaSuccess &&
+                         cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                         cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) == cudaSuccess && clusters > 0;
+        if (!can) cudaGetLastError();
+        answer = can ? 2 : 1;
+        known[device].store(answer, std::memory_order_relaxed);
+    }
+    return answer == 2;
+}
+
+cudaError_t launch_sort(SortArguments a, cudaStream_t stream) {
+    const long long pieces = (a.clear_bytes + kClearBytes - 1) / kClearBytes;
+    if (pieces > 2147483000ll) return cudaErrorInvalidValue;
+    if (a.count <= kSmallSort) {
+        int padded = 64;
+        while (padded < static_cast<int>(a.count)) padded <<= 1;
+        embedding_small_sort_kernel<<<static_cast<unsigned>(1 + pieces), kSortThreads, 0, stream>>>(a, padded);
+        return cudaPeekAtLastError();
+    }
+    a.passes = 1;                                // over the bits of the largest key, `vocab`
+    while (a.tokens.vocab >> (kDigitBits * a.passes) != 0) ++a.passes;
+    if (pieces > 0) {
+        const long long ctas = kClusterSmall + (pieces + kClusterSmall - 1) / kClusterSmall * kClusterSmall;
+        return launch_cluster<kClusterSmall>(embedding_sort_kernel<kClusterSmall, true>, ctas, a, stream);
+    }
+    if (a.count > kClusterSmall * kSortThreads * kSteps && large_clusters())
+        return launch_cluster<kClusterLarge>(embedding_sort_kernel<kClusterLarge, false>, kClusterLarge, a, stream);
+    return launch_cluster<kClusterSmall>(embedding_sort_kernel<kClusterSmall, false>, kClusterSmall, a, stream);
+}
+
+template <typename G, typename T, bool kVector>
+cudaError_t run_rows(RowsArguments a, cudaStream_t stream) {
+    constexpr int kValues = lane_values<G, kVector>();
+    const long long slices = (a.width + kValues * 32 - 1) / (kValues * 32);
+    if (a.chunks * slices > 2147483647ll) return cudaErrorInvalidValue;
+    a.slices = static_cast<int>(slices);
+    a.row_ctas = static_cast<int>((a.chunks * slices + kWarpsPerCta - 1) / kWarpsPerCta);
+    const bool join = a.chunks > 1;
+    a.join_groups = join ? a.late_groups - a.late_groups / 3 : a.late_groups;
+    const cudaError_t e = launch_dependent(embedding_rows_kernel<G, T, kVector>, a.row_ctas + static_cast<int>(a.join_groups),
+                                           kThreads, 0, stream, a);
+    if (e != cudaSuccess || !join) return e;
+    a.long_ctas = a.chunks > kLongChunks ? grid_for(a.chunks / kLongChunks * slices, 2) : 0;
+    a.join_ctas = a.long_ctas + grid_for(((a.chunks - 1) * slices + kWarpsPerCta - 1) / kWarpsPerCta, 4);
+    return launch_dependent(embedding_join_kernel<T, kValues, kVector>, a.join_ctas + static_cast<int>(a.late_groups - a.join_groups),
+                            kThreads, 0, stream, a);
 }
 
 template <typename G, typename T>
-cudaError_t run_rows(const RowsArguments& a, bool vector_ok, int grid, cudaStream_t stream) {
-    cudaError_t e = vector_ok ? launch_dependent(embedding_rows_kernel<G, T, true>, grid, kThreads, 0, stream, a)
-                              : launch_dependent(embedding_rows_kernel<G, T, false>, grid, kThreads, 0, stream, a);
-    if (e != cudaSuccess || a.chunks < 2) return e;
-    const int join = grid_for(static_cast<long long>(a.chunks - 1) * a.slices, 4);
-    return vector_ok ? launch_dependent(embedding_join_kernel<T, true>, join, kThreads, 0, stream, a)
-                     : launch_dependent(embedding_join_kernel<T, false>, join, kThreads, 0, stream, a);
+cudaError_t run_rows(const RowsArguments& a, bool vector_ok, cudaStream_t stream) {
+    return vector_ok ? run_rows<G, T, true>(a, stream) : run_rows<G, T, false>(a, stream);
 }
 
 int gradient(int device, int gradient_kind, const void* out_gradient, long long gradient_stride, const void* tokens,
@@ -664,42 +889,57 @@ int gradient(int device, int gradient_kind, const void* out_gradient, long long 
         (count > 0 && (!tokens || !out_gradient)))
         return static_cast<int>(cudaErrorInvalidValue);
     const GradientScratch s = gradient_scratch(count, vocab, width);
-    const int slices = (width + kSliceColumns - 1) / kSliceColumns;
-    const long long row_ctas = (s.chunks * slices + kWarpsPerCta - 1) / kWarpsPerCta;
-    const long long zero_ctas = accumulate ? 0 : (vocab + kZeroRows - 1) / kZeroRows;
     const int gradient_bytes = gradient_kind == 0 ? 4 : 2, table_bytes = table_kind == 0 ? 4 : 2;
     if (!aligned_for(out_gradient, gradient_bytes) || !aligned_for(table_gradient, table_bytes) ||
         !aligned_for(tokens, token_bytes) || !aligned_for(token_status, 4) || !workspace || !aligned_for(workspace, 16) ||
-        workspace_bytes < s.bytes || row_ctas + zero_ctas > 2147483647ll || s.chunks * slices > 2147483647ll)
+        workspace_bytes < s.bytes)
         return static_cast<int>(cudaErrorInvalidValue);
     if (count == 0 && accumulate) return static_cast<int>(cudaSuccess);
     const DeviceScope scope(device);
     if (scope.status() != cudaSuccess) return scope.status();
     char* scratch = static_cast<char*>(workspace);
-    auto words = [&](long long at) { return reinterpret_cast<unsigned*>(scratch + at); };
-    int key_bits = 0;                            // of the largest key, `vocab`
-    while ((vocab >> key_bits) != 0) ++key_bits;
-    const int passes = (key_bits + kDigitBits - 1) / kDigitBits;
-    const SortArguments sort{Tokens{tokens, token_bytes, padding_token, vocab}, {words(s.keys[0]), words(s.keys[1])},
-                             {words(s.positions[0]), words(s.positions[1])}, accumulate ? nullptr : words(s.touched),
-                             words(s.crossing), token_status, static_cast<unsigned>(count), passes,
-                             (key_bits + passes - 1) / passes};
+    SortArguments sort{};
+    sort.tokens = Tokens{tokens, token_bytes, padding_token, vocab};
+    for (int i = 0; i < 2; ++i) sort.pairs[i] = reinterpret_cast<uint2*>(scratch + s.pairs[i]);
+    sort.crossing = reinterpret_cast<unsigned*>(scratch + s.crossing);
+    sort.status = token_status;
+    // A quarter of the zeros, 128 MB at most, is left to the rows and join launches, which have their own short waits.
+    const long long row_bytes = static_cast<long long>(width) * table_bytes;
+    long long late_rows = kLateBytes / row_bytes < vocab / 4 ? kLateBytes / row_bytes : vocab / 4;
+    if (accumulate || count == 0) late_rows = 0;
+    if (late_rows > 0) sort.named = reinterpret_cast<unsigned*>(scratch + s.named);
+    sort.clear = static_cast<char*>(table_gradient);
+    sort.clear_bytes = accumulate ? 0 : (vocab - late_rows) * row_bytes;
+    sort.count = static_cast<unsigned>(count);
     cudaError_t e = launch_sort(sort, stream);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    const RowsArguments a{words(s.keys[0]), words(s.positions[0]), words(s.touched), words(s.crossing),
-                          reinterpret_cast<float*>(scratch + s.tails), reinterpret_cast<float*>(scratch + s.heads),
-                          out_gradient, table_gradient, gradient_stride, static_cast<unsigned>(count),
-                          static_cast<unsigned>(vocab), static_cast<unsigned>(s.chunks), width, slices,
-                          static_cast<int>(row_ctas), scale, accumulate != 0};
+    if (e != cudaSuccess || count == 0) return static_cast<int>(e);
+    RowsArguments a{};
+    a.pairs = sort.pairs[0];
+    a.crossing = sort.crossing;
+    a.crossing_short = reinterpret_cast<unsigned*>(scratch + s.crossing_short);
+    a.crossing_long = reinterpret_cast<unsigned*>(scratch + s.crossing_long);
+    a.tails = reinterpret_cast<float*>(scratch + s.tails);
+    a.heads = reinterpret_cast<float*>(scratch + s.heads);
+    a.gradient = out_gradient;
+    a.table = table_gradient;
+    a.gradient_stride = gradient_stride;
+    a.count = static_cast<unsigned>(count);
+    a.vocab = static_cast<unsigned>(vocab);
+    a.chunks = static_cast<unsigned>(s.chunks);
+    a.width = width;
+    a.scale = scale;
+    a.accumulate = accumulate != 0;
+    a.named = sort.named;
+    a.late = vocab - late_rows;
+    a.late_groups = static_cast<unsigned>((late_rows + kZeroRows - 1) / kZeroRows);
+    a.chunk = static_cast<unsigned>(s.chunk);
     const bool vector_ok = width % 8 == 0 && aligned_for(out_gradient, 16) && gradient_stride * gradient_bytes % 16 == 0 &&
                            aligned_for(table_gradient, 16);
-    const int grid = static_cast<int>(row_ctas + zero_ctas);
     if (gradient_kind == 0)
-        e = table_kind == 0 ? run_rows<float, float>(a, vector_ok, grid, stream)
-                            : run_rows<float, unsigned short>(a, vector_ok, grid, stream);
+        e = table_kind == 0 ? run_rows<float, float>(a, vector_ok, stream) : run_rows<float, unsigned short>(a, vector_ok, stream);
     else
-        e = table_kind == 0 ? run_rows<unsigned short, float>(a, vector_ok, grid, stream)
-                            : run_rows<unsigned short, unsigned short>(a, vector_ok, grid, stream);
+        e = table_kind == 0 ? run_rows<unsigned short, float>(a, vector_ok, stream)
+                            : run_rows<unsigned short, unsigned short>(a, vector_ok, stream);
     return static_cast<int>(e);
 }
 

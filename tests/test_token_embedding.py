@@ -52,10 +52,12 @@ def test_scratch_size(lib):
         assert lib.nntrain_embedding_gradient_workspace(count, vocab, width, ctypes.addressof(out)) == 0
         return out.value
 
-    # four arrays of a word per token, a bit per row, a word and two rows of fp32 per 32 tokens
-    for count, vocab, width in ((0, 1, 1), (1, 10, 64), (32, 10, 64), (33, 10, 64), (8192, 151936, 1536)):
-        chunks = -(-count // 32)
-        parts = [count * 4] * 4 + [-(-vocab // 32) * 4, (chunks + 1) * 4] + [chunks * width * 4] * 2
+    # two arrays of a pair per token, a bit per row, two counters, lists of the tokens that cross chunks of 16 or 32,
+    # two rows of fp32 a chunk
+    for count, vocab, width, chunk in ((0, 1, 1, 16), (1, 10, 64, 16), (32, 10, 64, 16), (33, 10, 64, 16),
+                                       (8192, 151936, 1536, 16), (65536, 32000, 512, 32)):
+        chunks = -(-count // chunk)
+        parts = [count * 8] * 2 + [-(-vocab // 32) * 4, 8, chunks * 4, (chunks // 16 + 1) * 4] + [chunks * width * 4] * 2
         assert size(count, vocab, width) == sum(-(-p // 256) * 256 for p in parts)
     for bad in ((-1, 10, 10), (10, 0, 10), (10, 10, 0), (1 << 31, 10, 10)):
         assert lib.nntrain_embedding_gradient_workspace(*bad, ctypes.addressof(out)) == INVALID

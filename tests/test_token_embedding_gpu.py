@@ -2,7 +2,7 @@
 
 Tolerances, with e = 2^-24.  Lookup: the decode's product and the scale's, then
 the output's rounding: bit for bit against the same products in numpy.
-Gradient: a row's n terms are added in fp32, 32 positions, then the chunks'
+Gradient: a row's n terms are added in fp32, up to 32 positions, then the chunks'
 partials, an eighth of them a warp: no term passes more than 32 + chunks + 8
 additions, each off by e of at most the sum of the absolute terms; the scale
 and the sum with what is there add 2 e, the output's rounding its half step."""
@@ -138,7 +138,7 @@ def check_gradient(tokens, dout, got, scale, vocab, before=None):
     np.add.at(size, tokens[valid], np.abs(d[valid]))
     counts = np.bincount(tokens[valid], minlength=vocab)
     want, size = want * scale, size * abs(scale)
-    bound = (32 + counts / 32 + 8 + 3)[:, None] * E * size
+    bound = (32 + counts / 16 + 8 + 3)[:, None] * E * size
     if before is not None:
         want = want + to_f64(before)
         bound = bound + E * (np.abs(want) + size) * (counts > 0)[:, None]
@@ -191,13 +191,33 @@ def test_every_number_of_passes_sorts(cuda, vocab):
         for i in range(len(t)):
             partial = (partial + d[i]).astype(np.float32)
             ends = i + 1 == len(t) or t[i + 1] != t[i]
-            if ends or (i + 1) % 32 == 0:                # a chunk's border splits the sum
+            if ends or (i + 1) % 16 == 0:                # a chunk's border splits the sum
                 want[t[i]] = partial if at == 0 else (want[t[i]] + partial).astype(np.float32)
                 at = 0 if ends else 1
                 partial = np.zeros(width, np.float32)
         assert_bits_equal(host(got).ravel(), want.ravel(), "rows")
     else:
         check_gradient(tokens, dev(dout), got, 1.0, vocab)
+
+
+@pytest.mark.parametrize("vocab,width", ((70000, 4), (300_000, 4), (1 << 28, 1)))
+def test_one_bucket_takes_all(cuda, vocab, width):
+    """Rows that agree in their low 9 bits: one, two and three passes over the others."""
+    rng = np.random.default_rng(vocab)
+    count = 5000
+    rows = np.unique(np.concatenate([rng.integers(0, vocab // 512, 40), [0, vocab // 512 - 1]])) * 512
+    tokens = rows[rng.integers(0, len(rows), count)]
+    dout = rng.standard_normal((count, width)).astype(np.float32)
+    got = torch.full((vocab, width), 9.0, device="cuda")
+    TokenEmbedding.gradient(0, dev(tokens), dev(dout), got)
+    torch.cuda.synchronize()
+    want, size = np.zeros((len(rows), width)), np.zeros((len(rows), width))
+    np.add.at(want, np.searchsorted(rows, tokens), dout.astype(np.float64))
+    np.add.at(size, np.searchsorted(rows, tokens), np.abs(dout.astype(np.float64)))
+    index = torch.from_numpy(rows).cuda()
+    assert (np.abs(to_f64(got[index]) - want) <= (32 + count / 16 + 8 + 3) * E * size).all()
+    got[index] = 0.0
+    assert not got.any()
 
 
 def test_same_inputs_same_bits(cuda):
