@@ -35,7 +35,7 @@ namespace {
 constexpr int kRowThreads = 512;              // most threads on a row held in registers
 constexpr int kLoopThreads = 256;             // threads on a row that is not
 constexpr int kMostPartials = 1184;           // most CTAs that leave a partial weight gradient: 8 on each of 148 SMs
-constexpr int kJoinColumns = 32, kJoinRows = 32;
+constexpr int kJoinColumns = 8, kJoinRows = 64;   // 32 bytes of a partial, a sector
 
 struct RowSum {
     float (*slots)[kRowThreads / 32];
@@ -65,26 +65,77 @@ __device__ __forceinline__ float over_cta(float v, RowSum& s) {
 
 // ---- loads and stores of a group -------------------------------------------------
 
-template <int kVec>
-__device__ __forceinline__ void load_group(const float* p, float (&v)[kVec]) {
+// A group as it lies in memory, so that the next row's can be on its way while
+// this row is worked on.
+template <typename T, int kVec>
+struct Raw {
+    T value;
+};
+template <typename T>
+struct Raw<T, 8> {
+    uint4 words[sizeof(T) / 2];
+};
+
+template <typename T, int kVec>
+__device__ __forceinline__ void load_raw(const T* p, Raw<T, kVec>& raw) {
     if constexpr (kVec == 1) {
-        v[0] = *p;
+        raw.value = *p;
     } else {
-        const float4 a = load_f4(p), b = load_f4(p + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        #pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) raw.words[i] = reinterpret_cast<const uint4*>(p)[i];
     }
 }
-template <int kVec>
-__device__ __forceinline__ void load_group(const unsigned short* p, float (&v)[kVec]) {
+
+template <typename T, int kVec>
+__device__ __forceinline__ void unpack(const Raw<T, kVec>& raw, float (&v)[kVec]) {
     if constexpr (kVec == 1) {
-        v[0] = bf16_value(*p);
+        if constexpr (sizeof(T) == 4) v[0] = raw.value;
+        else v[0] = bf16_value(raw.value);
     } else {
-        const uint4 a = *reinterpret_cast<const uint4*>(p);
-        v[0] = bf16_low(a.x); v[1] = bf16_high(a.x); v[2] = bf16_low(a.y); v[3] = bf16_high(a.y);
-        v[4] = bf16_low(a.z); v[5] = bf16_high(a.z); v[6] = bf16_low(a.w); v[7] = bf16_high(a.w);
+        #pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+            const uint4 w = raw.words[i];
+            if constexpr (sizeof(T) == 4) {
+                v[4 * i] = __uint_as_float(w.x); v[4 * i + 1] = __uint_as_float(w.y);
+                v[4 * i + 2] = __uint_as_float(w.z); v[4 * i + 3] = __uint_as_float(w.w);
+            } else {
+                v[0] = bf16_low(w.x); v[1] = bf16_high(w.x); v[2] = bf16_low(w.y); v[3] = bf16_high(w.y);
+                v[4] = bf16_low(w.z); v[5] = bf16_high(w.z); v[6] = bf16_low(w.w); v[7] = bf16_high(w.w);
+            }
+        }
     }
 }
+
+// First column of the thread's group g: a warp has 32 * kGroups neighbouring
+// groups, so the groups of a thread are a constant distance apart.
+template <int kVec, int kGroups>
+__device__ __forceinline__ int column_of(int g) {
+    return ((static_cast<int>(threadIdx.x) & ~31) * kGroups + g * 32 + (static_cast<int>(threadIdx.x) & 31)) * kVec;
+}
+
+// A row's groups of this thread; columns beyond the width are left alone.
+template <typename T, int kVec, int kGroups>
+__device__ __forceinline__ void load_row(const void* base, long long row, long long stride, int width, Raw<T, kVec> (&raw)[kGroups]) {
+    const T* p = static_cast<const T*>(base) + row * stride;
+    #pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+        if (column_of<kVec, kGroups>(g) < width) load_raw<T, kVec>(p + column_of<kVec, kGroups>(0) + g * 32 * kVec, raw[g]);
+    }
+}
+
+// Whether the next row is loaded ahead: where the raw groups of `inputs` rows are
+// few registers, so that they do not cost resident CTAs.
+template <typename T, int kVec, int kGroups>
+__host__ __device__ constexpr bool loads_ahead(int inputs) {
+    return kVec == 8 && inputs * kGroups * 2 * static_cast<int>(sizeof(T)) <= 16;
+}
+
+template <typename T>
+__device__ __forceinline__ float load_value(const T* p) {
+    if constexpr (sizeof(T) == 4) return *p;
+    else return bf16_value(*p);
+}
+
 template <int kVec>
 __device__ __forceinline__ void store_group(float* p, const float (&v)[kVec]) {
     if constexpr (kVec == 1) {
@@ -107,6 +158,33 @@ __device__ __forceinline__ float load_weight(const void* weight, int kind, long 
     return kind == 0 ? static_cast<const float*>(weight)[i] : bf16_value(static_cast<const unsigned short*>(weight)[i]);
 }
 
+// The weight's group at `column`: 128-bit loads where the weight lies on 16 bytes
+// (it is a view of a parameter arena and need not).
+template <int kVec>
+__device__ __forceinline__ void load_weights(const void* weight, int kind, bool aligned, int column, float (&w)[kVec]) {
+    if constexpr (kVec == 8) {
+        if (aligned) {
+            if (kind == 0) {
+                Raw<float, 8> raw;
+                load_raw<float, 8>(static_cast<const float*>(weight) + column, raw);
+                unpack<float, 8>(raw, w);
+            } else {
+                Raw<unsigned short, 8> raw;
+                load_raw<unsigned short, 8>(static_cast<const unsigned short*>(weight) + column, raw);
+                unpack<unsigned short, 8>(raw, w);
+            }
+            return;
+        }
+    }
+    #pragma unroll
+    for (int i = 0; i < kVec; ++i) w[i] = load_weight(weight, kind, column + i);
+}
+
+// Whether a thread keeps its weights in registers from row to row; with more of
+// them they would spill, and come from L1 for each row instead.
+template <int kVec, int kGroups>
+__host__ __device__ constexpr bool keeps_weights() { return kVec * kGroups <= 16; }
+
 // ---- forward ------------------------------------------------------------------
 
 struct ForwardArguments {
@@ -121,6 +199,7 @@ struct ForwardArguments {
     int* finite_status;                // null: not raised
     long long rows, x_stride, residual_stride;
     int width, block, weight_kind, y_kind;
+    bool weight_aligned;
     float epsilon;
 };
 
@@ -162,46 +241,47 @@ __global__ void __launch_bounds__(kRowThreads)
 rms_norm_forward_kernel(ForwardArguments a) {
     __shared__ float slots[2][kRowThreads / 32];
     RowSum sums{slots, 0};
-    const int threads = blockDim.x;
-    float w[kGroups][kVec];
-    #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-        const int column = (g * threads + threadIdx.x) * kVec;
-        #pragma unroll
-        for (int i = 0; i < kVec; ++i) w[g][i] = column < a.width ? load_weight(a.weight, a.weight_kind, column + i) : 0.0f;
-    }
-    bool bad = false;
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-        const long long base = row * a.width;
-        float h[kGroups][kVec];
+    constexpr bool kKeep = keeps_weights<kVec, kGroups>();
+    float kept[kKeep ? kGroups : 1][kVec] = {};
+    if (kKeep) {
         #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
-            const int column = (g * threads + threadIdx.x) * kVec;
-            if (column < a.width) {
-                load_group<kVec>(x + column, h[g]);
-            } else {
-                #pragma unroll
-                for (int i = 0; i < kVec; ++i) h[g][i] = 0.0f;
-            }
+            const int column = column_of<kVec, kGroups>(g);
+            if (column < a.width) load_weights<kVec>(a.weight, a.weight_kind, a.weight_aligned, column, kept[kKeep ? g : 0]);
         }
-        if (a.residual != nullptr) {
-            const T* residual = static_cast<const T*>(a.residual) + row * a.residual_stride;
+    }
+    constexpr bool kAhead = loads_ahead<T, kVec, kGroups>(2);
+    Raw<T, kVec> x[kGroups], r[kGroups];
+    auto load = [&](long long row) {
+        load_row<T, kVec, kGroups>(a.x, row, a.x_stride, a.width, x);
+        if (a.residual != nullptr) load_row<T, kVec, kGroups>(a.residual, row, a.residual_stride, a.width, r);
+    };
+    bool bad = false;
+    float not_finite = 0.0f;                     // NaN once a y is not finite: y * 0 is 0 or NaN
+    if (kAhead && blockIdx.x < a.rows) load(blockIdx.x);
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const long long base = row * a.width;
+        float h[kGroups][kVec];
+        if (!kAhead) load(row);
+        #pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            const int column = column_of<kVec, kGroups>(g);
             #pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-                const int column = (g * threads + threadIdx.x) * kVec;
-                if (column < a.width) {
-                    float r[kVec];
-                    load_group<kVec>(residual + column, r);
-                    #pragma unroll
-                    for (int i = 0; i < kVec; ++i) h[g][i] = __fadd_rn(h[g][i], r[i]);
-                }
+            for (int i = 0; i < kVec; ++i) h[g][i] = 0.0f;
+            if (column >= a.width) continue;
+            unpack<T, kVec>(x[g], h[g]);
+            if (a.residual != nullptr) {
+                float v[kVec];
+                unpack<T, kVec>(r[g], v);
+                #pragma unroll
+                for (int i = 0; i < kVec; ++i) h[g][i] = __fadd_rn(h[g][i], v[i]);
             }
         }
+        if (kAhead && row + gridDim.x < a.rows) load(row + gridDim.x);
         float squares = 0.0f;
         #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
-            const int column = (g * threads + threadIdx.x) * kVec;
+            const int column = column_of<kVec, kGroups>(g);
             if (a.residual_out != nullptr && column < a.width)
                 store_group<kVec>(static_cast<T*>(a.residual_out) + base + column, h[g]);
             #pragma unroll
@@ -212,10 +292,13 @@ rms_norm_forward_kernel(ForwardArguments a) {
         float largest = 0.0f;
         #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
+            const int column = column_of<kVec, kGroups>(g);
+            float w[kVec] = {};
+            if (!kKeep && column < a.width) load_weights<kVec>(a.weight, a.weight_kind, a.weight_aligned, column, w);
             #pragma unroll
             for (int i = 0; i < kVec; ++i) {
-                h[g][i] = __fmul_rn(__fmul_rn(h[g][i], inverse), w[g][i]);
-                bad |= is_non_finite(h[g][i]);
+                h[g][i] = __fmul_rn(__fmul_rn(h[g][i], inverse), kKeep ? kept[kKeep ? g : 0][i] : w[i]);
+                not_finite = __fmaf_rn(h[g][i], 0.0f, not_finite);
                 if (kBlock == 0) largest = fmaxf(largest, fabsf(h[g][i]));
             }
         }
@@ -224,9 +307,24 @@ rms_norm_forward_kernel(ForwardArguments a) {
             row_scale = scale_from_maximum_fast(over_cta<true>(largest, sums));
             if (threadIdx.x == 0) a.scales[row] = row_scale;
         }
+        if constexpr (kVec == 1 && kBlock == 0) {
+            // single values of one block: codes of four at a time, as of a group
+            const BlockScale divisor = block_scale(row_scale);
+            #pragma unroll
+            for (int g = 0; g < kGroups; g += 4) {
+                float t[4];
+                biased_codes_of(make_float4(h[g][0], h[g + 1][0], h[g + 2][0], h[g + 3][0]), divisor, t[0], t[1], t[2], t[3]);
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int column = column_of<1, kGroups>(g + i);
+                    if (column < a.width) a.payload[base + column] = code_byte(t[i]);
+                    h[g + i][0] = __fmul_rn(code_value(t[i]), row_scale);
+                }
+            }
+        }
         #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
-            const int column = (g * threads + threadIdx.x) * kVec;
+            const int column = column_of<kVec, kGroups>(g);
             if constexpr (kBlock > 0) {
                 constexpr int kLanes = kBlock / kVec;
                 float maximum = 0.0f;
@@ -237,12 +335,13 @@ rms_norm_forward_kernel(ForwardArguments a) {
                     if (threadIdx.x % kLanes == 0) a.scales[(base + column) / kBlock] = scale;
                     encode_group<kVec>(h[g], scale, a.payload + base + column);
                 }
-            } else if constexpr (kBlock == 0) {
+            } else if constexpr (kBlock == 0 && kVec == 8) {
                 if (column < a.width) encode_group<kVec>(h[g], row_scale, a.payload + base + column);
             }
             if (a.y != nullptr && column < a.width) store_y<kVec>(a.y, a.y_kind, base + column, h[g]);
         }
     }
+    bad |= !(not_finite == 0.0f);
     if (a.finite_status != nullptr && __any_sync(0xffffffffu, bad) && (threadIdx.x & 31) == 0)
         atomicExch(a.finite_status, 1);
 }
@@ -264,14 +363,8 @@ rms_norm_forward_loop_kernel(ForwardArguments a) {
         const T* residual = a.residual == nullptr ? nullptr : static_cast<const T*>(a.residual) + row * a.residual_stride;
         const long long base = row * a.width;
         auto h_at = [&](int i) {
-            float v[1];
-            load_group<1>(x + i, v);
-            if (residual != nullptr) {
-                float r[1];
-                load_group<1>(residual + i, r);
-                v[0] = __fadd_rn(v[0], r[0]);
-            }
-            return v[0];
+            const float v = load_value(x + i);
+            return residual != nullptr ? __fadd_rn(v, load_value(residual + i)) : v;
         };
         float squares = 0.0f;
         for (int i = threadIdx.x; i < a.width; i += kLoopThreads) {
@@ -326,6 +419,7 @@ struct BackwardArguments {
     float* partials;                   // [CTAs][width]
     long long rows, y_stride, residual_stride, h_stride;
     int width, weight_kind;
+    bool weight_aligned;
 };
 
 template <typename T, int kVec, int kGroups>
@@ -333,66 +427,77 @@ __global__ void __launch_bounds__(kRowThreads)
 rms_norm_backward_kernel(BackwardArguments a) {
     __shared__ float slots[2][kRowThreads / 32];
     RowSum sums{slots, 0};
-    const int threads = blockDim.x;
-    float w[kGroups][kVec], dw[kGroups][kVec];
-    #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-        const int column = (g * threads + threadIdx.x) * kVec;
+    let_next_start();
+    constexpr bool kKeep = keeps_weights<kVec, kGroups>();
+    float kept[kKeep ? kGroups : 1][kVec] = {}, dw[kGroups][kVec] = {};
+    if (kKeep) {
         #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-            w[g][i] = column < a.width ? load_weight(a.weight, a.weight_kind, column + i) : 0.0f;
-            dw[g][i] = 0.0f;
+        for (int g = 0; g < kGroups; ++g) {
+            const int column = column_of<kVec, kGroups>(g);
+            if (column < a.width) load_weights<kVec>(a.weight, a.weight_kind, a.weight_aligned, column, kept[kKeep ? g : 0]);
         }
     }
     const float width = static_cast<float>(a.width);
+    constexpr bool kAhead = loads_ahead<T, kVec, kGroups>(3);
+    Raw<T, kVec> dy[kGroups], h[kGroups], r[kGroups];
+    float inverse_ahead = 0.0f;
+    auto load = [&](long long row) {
+        load_row<T, kVec, kGroups>(a.y_gradient, row, a.y_stride, a.width, dy);
+        load_row<T, kVec, kGroups>(a.h, row, a.h_stride, a.width, h);
+        if (kAhead && a.residual_gradient != nullptr)
+            load_row<T, kVec, kGroups>(a.residual_gradient, row, a.residual_stride, a.width, r);
+        inverse_ahead = a.inverse_rms[row];
+    };
+    if (kAhead && blockIdx.x < a.rows) load(blockIdx.x);
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const T* dy = static_cast<const T*>(a.y_gradient) + row * a.y_stride;
-        const T* h = static_cast<const T*>(a.h) + row * a.h_stride;
-        const float inverse = a.inverse_rms[row];
+        if (!kAhead) load(row);
+        const float inverse = inverse_ahead;
         float d[kGroups][kVec], n[kGroups][kVec];
-        #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-            const int column = (g * threads + threadIdx.x) * kVec;
-            if (column < a.width) {
-                load_group<kVec>(dy + column, d[g]);
-                load_group<kVec>(h + column, n[g]);
-            } else {
-                #pragma unroll
-                for (int i = 0; i < kVec; ++i) d[g][i] = n[g][i] = 0.0f;
-            }
-        }
         float along = 0.0f;
         #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
+            const int column = column_of<kVec, kGroups>(g);
+            #pragma unroll
+            for (int i = 0; i < kVec; ++i) d[g][i] = n[g][i] = 0.0f;
+            if (column < a.width) {
+                unpack<T, kVec>(dy[g], d[g]);
+                unpack<T, kVec>(h[g], n[g]);
+            }
+            float w[kVec] = {};
+            if (!kKeep && column < a.width) load_weights<kVec>(a.weight, a.weight_kind, a.weight_aligned, column, w);
             #pragma unroll
             for (int i = 0; i < kVec; ++i) {
                 n[g][i] = __fmul_rn(n[g][i], inverse);
                 dw[g][i] = __fmaf_rn(d[g][i], n[g][i], dw[g][i]);
-                d[g][i] = __fmul_rn(d[g][i], w[g][i]);
+                d[g][i] = __fmul_rn(d[g][i], kKeep ? kept[kKeep ? g : 0][i] : w[i]);
                 along = __fmaf_rn(d[g][i], n[g][i], along);
             }
+        }
+        Raw<T, kVec> added[kGroups];
+        if (kAhead) {
+            #pragma unroll
+            for (int g = 0; g < kGroups; ++g) added[g] = r[g];
+            if (row + gridDim.x < a.rows) load(row + gridDim.x);
         }
         const float mean = __fdiv_rn(over_cta<false>(along, sums), width);
         #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
-            const int column = (g * threads + threadIdx.x) * kVec;
+            const int column = column_of<kVec, kGroups>(g);
             if (column >= a.width) continue;
-            float r[kVec];
+            float v[kVec] = {};
             if (a.residual_gradient != nullptr) {
-                load_group<kVec>(static_cast<const T*>(a.residual_gradient) + row * a.residual_stride + column, r);
-            } else {
-                #pragma unroll
-                for (int i = 0; i < kVec; ++i) r[i] = 0.0f;
+                if (!kAhead) load_raw<T, kVec>(static_cast<const T*>(a.residual_gradient) + row * a.residual_stride + column, added[g]);
+                unpack<T, kVec>(added[g], v);
             }
             #pragma unroll
-            for (int i = 0; i < kVec; ++i) d[g][i] = __fmaf_rn(inverse, __fmaf_rn(-n[g][i], mean, d[g][i]), r[i]);
+            for (int i = 0; i < kVec; ++i) d[g][i] = __fmaf_rn(inverse, __fmaf_rn(-n[g][i], mean, d[g][i]), v[i]);
             store_group<kVec>(static_cast<T*>(a.x_gradient) + row * a.width + column, d[g]);
         }
     }
     float* partial = a.partials + static_cast<long long>(blockIdx.x) * a.width;
     #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
-        const int column = (g * threads + threadIdx.x) * kVec;
+        const int column = column_of<kVec, kGroups>(g);
         #pragma unroll
         for (int i = 0; i < kVec; ++i)
             if (column < a.width) partial[column + i] = dw[g][i];
@@ -414,31 +519,26 @@ rms_norm_backward_loop_kernel(BackwardArguments a) {
         const float inverse = a.inverse_rms[row];
         float along = 0.0f;
         for (int i = threadIdx.x; i < a.width; i += kLoopThreads) {
-            float d[1], n[1];
-            load_group<1>(dy + i, d);
-            load_group<1>(h + i, n);
-            n[0] = __fmul_rn(n[0], inverse);
-            partial[i] = __fmaf_rn(d[0], n[0], partial[i]);
-            along = __fmaf_rn(__fmul_rn(d[0], load_weight(a.weight, a.weight_kind, i)), n[0], along);
+            const float d = load_value(dy + i), n = __fmul_rn(load_value(h + i), inverse);
+            partial[i] = __fmaf_rn(d, n, partial[i]);
+            along = __fmaf_rn(__fmul_rn(d, load_weight(a.weight, a.weight_kind, i)), n, along);
         }
         const float mean = __fdiv_rn(over_cta<false>(along, sums), static_cast<float>(a.width));
         for (int i = threadIdx.x; i < a.width; i += kLoopThreads) {
-            float d[1], n[1], r[1] = {0.0f};
-            load_group<1>(dy + i, d);
-            load_group<1>(h + i, n);
-            if (a.residual_gradient != nullptr)
-                load_group<1>(static_cast<const T*>(a.residual_gradient) + row * a.residual_stride + i, r);
-            const float g = __fmul_rn(d[0], load_weight(a.weight, a.weight_kind, i));
-            d[0] = __fmaf_rn(inverse, __fmaf_rn(-__fmul_rn(n[0], inverse), mean, g), r[0]);
-            store_group<1>(static_cast<T*>(a.x_gradient) + row * a.width + i, d);
+            const float g = __fmul_rn(load_value(dy + i), load_weight(a.weight, a.weight_kind, i));
+            const float n = __fmul_rn(load_value(h + i), inverse);
+            const float r = a.residual_gradient == nullptr
+                ? 0.0f : load_value(static_cast<const T*>(a.residual_gradient) + row * a.residual_stride + i);
+            const float dx[1] = {__fmaf_rn(inverse, __fmaf_rn(-n, mean, g), r)};
+            store_group<1>(static_cast<T*>(a.x_gradient) + row * a.width + i, dx);
         }
     }
 }
 
-// dw (+)= sum of the partials, in a fixed order: 32 threads share a column.
+// dw (+)= sum of the partials, in a fixed order: 64 threads share a column.
 __global__ void __launch_bounds__(kJoinColumns * kJoinRows)
 rms_norm_join_kernel(const float* partials, int count, int width, void* weight_gradient, int kind, bool accumulate) {
-    __shared__ float sums[kJoinRows][kJoinColumns + 1];
+    __shared__ float sums[kJoinRows][kJoinColumns];
     const int x = threadIdx.x % kJoinColumns, y = threadIdx.x / kJoinColumns;
     const int column = blockIdx.x * kJoinColumns + x;
     wait_for_previous();
@@ -448,19 +548,17 @@ rms_norm_join_kernel(const float* partials, int count, int width, void* weight_g
         for (int r = y; r < count; r += kJoinRows) sum = __fadd_rn(sum, partials[static_cast<long long>(r) * width + column]);
     }
     sums[y][x] = sum;
-    __syncthreads();
-    // warp y sums column y of the tile over its 32 rows
-    float total = sums[x][y];
-    #pragma unroll
-    for (int offset = 16; offset > 0; offset >>= 1) total = __fadd_rn(total, __shfl_xor_sync(0xffffffffu, total, offset));
-    const int mine = blockIdx.x * kJoinColumns + y;
-    if (x != 0 || mine >= width) return;
+    for (int half = kJoinRows / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (y < half) sums[y][x] = __fadd_rn(sums[y][x], sums[y + half][x]);
+    }
+    if (y != 0 || column >= width) return;
     if (kind == 0) {
-        float* out = static_cast<float*>(weight_gradient) + mine;
-        *out = accumulate ? __fadd_rn(*out, total) : total;
+        float* out = static_cast<float*>(weight_gradient) + column;
+        *out = accumulate ? __fadd_rn(*out, sums[0][x]) : sums[0][x];
     } else {
-        unsigned short* out = static_cast<unsigned short*>(weight_gradient) + mine;
-        *out = bf16_bits(accumulate ? __fadd_rn(bf16_value(*out), total) : total);
+        unsigned short* out = static_cast<unsigned short*>(weight_gradient) + column;
+        *out = bf16_bits(accumulate ? __fadd_rn(bf16_value(*out), sums[0][x]) : sums[0][x]);
     }
 }
 
@@ -500,7 +598,8 @@ RowShape row_shape(int units, long long rows) {
 template <typename T, int kVec, int kGroups, int kBlock>
 cudaError_t launch_forward(const ForwardArguments& a, int threads, cudaStream_t stream) {
     constexpr auto kKernel = rms_norm_forward_kernel<T, kVec, kGroups, kBlock>;
-    kKernel<<<resident_grid<kKernel>(threads, a.rows), threads, 0, stream>>>(a);
+    const int grid = resident_grid<kKernel>(threads, a.rows);
+    kKernel<<<grid, threads, 0, stream>>>(a);
     return cudaPeekAtLastError();
 }
 
@@ -589,7 +688,7 @@ int forward(int device, int kind, const void* x, long long x_stride, const void*
     const DeviceScope scope(device);
     if (scope.status() != cudaSuccess) return scope.status();
     const ForwardArguments a{x, residual, weight, residual_out, y, payload, scales, inverse_rms, finite_status,
-                             rows, x_stride, residual_stride, width, block, weight_kind, y_kind, epsilon};
+                             rows, x_stride, residual_stride, width, block, weight_kind, y_kind, aligned_for(weight, 16), epsilon};
     const bool vector_ok = width % 8 == 0 && rows_aligned(x, kind, x_stride) &&
                            (!residual || rows_aligned(residual, kind, residual_stride)) &&
                            aligned_for(residual_out, 16) && aligned_for(y, 16) && aligned_for(payload, 8);
@@ -616,7 +715,7 @@ int backward(int device, int kind, const void* y_gradient, long long y_stride, c
     cudaError_t e = cudaSuccess;
     if (rows > 0) {
         const BackwardArguments a{y_gradient, residual_gradient, h, weight, inverse_rms, x_gradient,
-                                  static_cast<float*>(workspace), rows, y_stride, residual_stride, h_stride, width, weight_kind};
+                                  static_cast<float*>(workspace), rows, y_stride, residual_stride, h_stride, width, weight_kind, aligned_for(weight, 16)};
         const bool vector_ok = width % 8 == 0 && rows_aligned(y_gradient, kind, y_stride) && rows_aligned(h, kind, h_stride) &&
                                (!residual_gradient || rows_aligned(residual_gradient, kind, residual_stride)) &&
                                aligned_for(x_gradient, 16);

@@ -17,6 +17,7 @@ buffers.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import numpy as np
 import torch
@@ -47,19 +48,22 @@ def _require(t: torch.Tensor, dtype, name: str, device: int | None = None) -> No
         raise ValueError(f"{name} is on device {t.device.index}, expected {device}")
 
 
+_F32 = torch.float32
 _FLOAT32, _BFLOAT16 = (torch.float32,), (torch.bfloat16, torch.int16)   # bf16 values, or their bits
 _FLOATS = _FLOAT32 + _BFLOAT16
+_INT32, _INT8, _INTEGERS = (torch.int32,), (torch.int8,), (torch.int64, torch.int32)
+_current_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _kind(t: torch.Tensor) -> int:
     """0 = fp32, 1 = bf16 (the kinds of the C boundary)."""
-    return 0 if t.dtype == torch.float32 else 1
+    return 0 if t.dtype is _F32 else 1
 
 
 def _stream_on(device: int, stream) -> int:
     """The handle of `stream`, or of the device's current stream."""
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream
+        return _current_raw_stream(device)
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
@@ -76,16 +80,61 @@ def _scratch(device: int, bytes_: int, stream):
         return torch.empty(bytes_, dtype=torch.uint8, device=torch.device("cuda", device))
 
 
-def _workspace(operation: str, bytes_of, sizes, device: int, given, stream):
-    """(scratch, its bytes) for one call: the caller's, or allocated for it."""
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(function: str, *sizes) -> int:
+    """What the library's host-only function says that a call of these sizes needs."""
     need = ctypes.c_longlong()
-    check(operation, bytes_of(*sizes, ctypes.addressof(need)))
+    check(function, getattr(load(), function)(*sizes, ctypes.addressof(need)))
+    return need.value
+
+
+def _workspace(function: str, sizes, device: int, given, stream):
+    """(scratch, its bytes) for one call: the caller's, or allocated for it."""
+    need = _scratch_bytes(function, *sizes)
     if given is None:
-        return _scratch(device, need.value, stream), need.value
+        return _scratch(device, need, stream), need
     _require(given, torch.uint8, "workspace", device)
-    if given.numel() < need.value:
-        raise ValueError(f"workspace has {given.numel()} bytes, needs {need.value}")
+    if given.numel() < need:
+        raise ValueError(f"workspace has {given.numel()} bytes, needs {need}")
     return given, given.numel()
+
+
+def _vector(t: torch.Tensor, name: str, device: int, length: int, dtypes) -> int:
+    """Checks a contiguous tensor of `length` values and returns its address."""
+    if not (t.dtype in dtypes and t.numel() == length and t.get_device() == device and t.is_contiguous()):
+        _require(t, t.dtype, name, device)
+        if t.dtype not in dtypes:
+            raise ValueError(f"{name} has type {t.dtype}, expected one of {', '.join(map(str, dtypes))}")
+        raise ValueError(f"{name} has {t.numel()} values, expected {length}")
+    return t.data_ptr()
+
+
+def _status(t, name: str, device: int) -> int:
+    """Checks an optional int32 flag and returns its address."""
+    if t is None:
+        return 0
+    if t.numel() < 1:
+        raise ValueError(f"{name} needs a value")
+    return _vector(t, name, device, t.numel(), _INT32)
+
+
+def _rows(t: torch.Tensor, name: str, device: int, width: int, dtypes, rows: int | None = None) -> int:
+    """Checks a matrix of rows (contiguous values, any row stride) and returns the stride."""
+    if t.get_device() != device:
+        raise ValueError(f"{name} must be on CUDA device {device}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} has type {t.dtype}, expected one of {', '.join(map(str, dtypes))}")
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != width or (rows is not None and shape[0] != rows):
+        raise ValueError(f"{name} has shape {tuple(shape)}, expected ({'rows' if rows is None else rows}, {width})")
+    row, value = t.stride()
+    if value != 1 and width > 1 and shape[0] > 0:
+        raise ValueError(f"{name}: the values of a row must be contiguous")
+    if shape[0] <= 1:
+        return width
+    if row < width:
+        raise ValueError(f"{name}: rows must not overlap")
+    return row
 
 
 def scale_count(length: int, block_size: int) -> int:
@@ -424,6 +473,7 @@ class GradientTensorList:
         self.device, self.count, self.chunks, self.chunk_values = device, count, chunks.value, values.value
         self.table = torch.from_numpy(table.view(np.uint8)).to(f"cuda:{device}")
         self.chunk_map = torch.from_numpy(chunk_map).to(f"cuda:{device}")
+        self.table_address, self.map_address = self.table.data_ptr(), self.chunk_map.data_ptr()
         self._held = (list(tensors), scales, destinations)
 
 
@@ -459,17 +509,17 @@ class GradientNorm:
         same time uses."""
         if tensors.device != device:
             raise ValueError(f"the list is on device {tensors.device}, expected {device}")
-        _require(norm_and_coefficient, torch.float32, "norm_and_coefficient", device)
         if norm_and_coefficient.numel() < 2:
             raise ValueError("norm_and_coefficient needs two values")
+        out = _vector(norm_and_coefficient, "norm_and_coefficient", device, norm_and_coefficient.numel(), _FLOAT32)
         if not max_norm > 0.0:
             raise ValueError("max_norm must be positive")
+        norms = 0
         if tensor_norms is not None:
-            _require(tensor_norms, torch.float32, "tensor_norms", device)
             if tensor_norms.numel() < tensors.count:
                 raise ValueError("tensor_norms needs one value for each tensor")
-        if finite_status is not None:
-            _require(finite_status, torch.int32, "finite_status", device)
+            norms = _vector(tensor_norms, "tensor_norms", device, tensor_norms.numel(), _FLOAT32)
+        status = _status(finite_status, "finite_status", device)
         if workspace is None:
             workspace = _scratch(device, tensors.chunks * 8, stream)
         else:
@@ -477,9 +527,9 @@ class GradientNorm:
             if workspace.numel() < tensors.chunks:
                 raise ValueError("workspace is too small")
         check("gradient_list_clip", load().nntrain_gradient_list_clip(
-            device, tensors.table.data_ptr(), tensors.count, tensors.chunk_map.data_ptr(), tensors.chunks,
-            tensors.chunk_values, _ptr(workspace), max_norm, int(apply), norm_and_coefficient.data_ptr(),
-            _ptr(tensor_norms), _ptr(finite_status), _stream_on(device, stream)))
+            device, tensors.table_address, tensors.count, tensors.map_address, tensors.chunks, tensors.chunk_values,
+            0 if workspace is None else workspace.data_ptr(), max_norm, apply, out, norms, status,
+            _stream_on(device, stream)))
 
 
 class Bfp8GradientOptimizers:
@@ -502,31 +552,6 @@ class Bfp8GradientOptimizers:
             scaled_epsilon, int(apply_weight_decay), _stream(stream)))
 
 
-def _rows(t: torch.Tensor, name: str, device: int, width: int, dtypes, rows: int | None = None) -> int:
-    """Checks a matrix of rows (contiguous values, any row stride) and returns the stride."""
-    if not t.is_cuda or t.device.index != device:
-        raise ValueError(f"{name} must be on CUDA device {device}")
-    if t.dtype not in dtypes:
-        raise ValueError(f"{name} has type {t.dtype}, expected one of {', '.join(map(str, dtypes))}")
-    if t.dim() != 2 or t.shape[1] != width or (rows is not None and t.shape[0] != rows):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({'rows' if rows is None else rows}, {width})")
-    if t.shape[0] <= 1:
-        if width > 1 and t.shape[0] == 1 and t.stride(1) != 1:
-            raise ValueError(f"{name}: the values of a row must be contiguous")
-        return width
-    if (width > 1 and t.stride(1) != 1) or t.stride(0) < width:
-        raise ValueError(f"{name}: the values of a row must be contiguous and rows must not overlap")
-    return t.stride(0)
-
-
-def _vector(t: torch.Tensor, name: str, device: int, length: int, dtypes) -> None:
-    _require(t, t.dtype, name, device)
-    if t.dtype not in dtypes:
-        raise ValueError(f"{name} has type {t.dtype}, expected one of {', '.join(map(str, dtypes))}")
-    if t.numel() != length:
-        raise ValueError(f"{name} has {t.numel()} values, expected {length}")
-
-
 class RmsNorm:
     """Root-mean-square norm of x + residual whose output goes to the codec's 8
     bits, and its gradient.  Matrices are (rows, width), fp32 or bf16 (bfloat16
@@ -543,32 +568,33 @@ class RmsNorm:
         if x.dim() != 2:
             raise ValueError(f"x has shape {tuple(x.shape)}, expected (rows, width)")
         rows, width = x.shape
-        same = _FLOAT32 if x.dtype == torch.float32 else _BFLOAT16
+        kind = _kind(x)
+        same = _BFLOAT16 if kind else _FLOAT32
         x_stride = _rows(x, "x", device, width, same)
-        residual_stride = 0 if residual is None else _rows(residual, "residual", device, width, same, rows)
-        _vector(weight, "weight", device, width, _FLOATS)
+        weight_address = _vector(weight, "weight", device, width, _FLOATS)
+        residual_stride = residual_address = h = inverse = y_address = y_kind = codes = scale_address = 0
+        if residual is not None:
+            residual_stride, residual_address = _rows(residual, "residual", device, width, same, rows), residual.data_ptr()
         if y is None and payload is None:
             raise ValueError("the norm needs an output: y, or payload and scales")
         if y is not None:
-            _vector(y, "y", device, rows * width, _FLOATS)
+            y_address, y_kind = _vector(y, "y", device, rows * width, _FLOATS), _kind(y)
         if residual_out is not None:
             if residual is None:
                 raise ValueError("residual_out without a residual is x itself")
-            _vector(residual_out, "residual_out", device, rows * width, same)
+            h = _vector(residual_out, "residual_out", device, rows * width, same)
         if payload is not None:
             block = width if block_size == 0 or block_size > width else block_size
             if block < 0 or scales is None or (width and width % block != 0):
                 raise ValueError("an encoded output needs scales and a block size that divides the width")
-            _vector(payload, "payload", device, rows * width, (torch.int8,))
-            _vector(scales, "scales", device, rows * (width // block) if width else 0, _FLOAT32)
+            codes = _vector(payload, "payload", device, rows * width, _INT8)
+            scale_address = _vector(scales, "scales", device, rows * (width // block) if width else 0, _FLOAT32)
         if inverse_rms is not None:
-            _vector(inverse_rms, "inverse_rms", device, rows, _FLOAT32)
-        if finite_status is not None:
-            _require(finite_status, torch.int32, "finite_status", device)
+            inverse = _vector(inverse_rms, "inverse_rms", device, rows, _FLOAT32)
         check("rms_norm_forward", load().nntrain_rms_norm_forward(
-            device, _kind(x), x.data_ptr(), x_stride, _ptr(residual), residual_stride, weight.data_ptr(), _kind(weight),
-            rows, width, epsilon, _ptr(residual_out), _ptr(y), 0 if y is None else _kind(y), _ptr(payload), _ptr(scales),
-            block_size, _ptr(inverse_rms), _ptr(finite_status), _stream_on(device, stream)))
+            device, kind, x.data_ptr(), x_stride, residual_address, residual_stride, weight_address, _kind(weight), rows,
+            width, epsilon, h, y_address, y_kind, codes, scale_address, block_size, inverse,
+            _status(finite_status, "finite_status", device), _stream_on(device, stream)))
 
     @staticmethod
     def backward(device: int, y_gradient, h, weight, inverse_rms, x_gradient, weight_gradient, residual_gradient=None,
@@ -582,21 +608,23 @@ class RmsNorm:
         if h.dim() != 2:
             raise ValueError(f"h has shape {tuple(h.shape)}, expected (rows, width)")
         rows, width = h.shape
-        same = _FLOAT32 if h.dtype == torch.float32 else _BFLOAT16
+        kind = _kind(h)
+        same = _BFLOAT16 if kind else _FLOAT32
         h_stride = _rows(h, "h", device, width, same)
         y_stride = _rows(y_gradient, "y_gradient", device, width, same, rows)
-        residual_stride = 0 if residual_gradient is None else _rows(residual_gradient, "residual_gradient", device, width, same, rows)
-        _vector(weight, "weight", device, width, _FLOATS)
-        _vector(inverse_rms, "inverse_rms", device, rows, _FLOAT32)
-        _vector(x_gradient, "x_gradient", device, rows * width, same)
-        _vector(weight_gradient, "weight_gradient", device, width, _FLOATS)
-        workspace, bytes_ = _workspace("rms_norm_backward", load().nntrain_rms_norm_backward_workspace, (rows, width), device,
-                                       workspace, stream)
+        residual_stride = residual_address = 0
+        if residual_gradient is not None:
+            residual_stride = _rows(residual_gradient, "residual_gradient", device, width, same, rows)
+            residual_address = residual_gradient.data_ptr()
+        weight_address = _vector(weight, "weight", device, width, _FLOATS)
+        inverse = _vector(inverse_rms, "inverse_rms", device, rows, _FLOAT32)
+        dx = _vector(x_gradient, "x_gradient", device, rows * width, same)
+        dw = _vector(weight_gradient, "weight_gradient", device, width, _FLOATS)
+        workspace, bytes_ = _workspace("nntrain_rms_norm_backward_workspace", (rows, width), device, workspace, stream)
         check("rms_norm_backward", load().nntrain_rms_norm_backward(
-            device, _kind(h), y_gradient.data_ptr(), y_stride, _ptr(residual_gradient), residual_stride, h.data_ptr(),
-            h_stride, weight.data_ptr(), _kind(weight), inverse_rms.data_ptr(), rows, width, x_gradient.data_ptr(),
-            weight_gradient.data_ptr(), _kind(weight_gradient), int(accumulate), _ptr(workspace), bytes_,
-            _stream_on(device, stream)))
+            device, kind, y_gradient.data_ptr(), y_stride, residual_address, residual_stride, h.data_ptr(), h_stride,
+            weight_address, _kind(weight), inverse, rows, width, dx, dw, _kind(weight_gradient), accumulate,
+            0 if workspace is None else workspace.data_ptr(), bytes_, _stream_on(device, stream)))
 
 
 class TokenEmbedding:
@@ -613,22 +641,21 @@ class TokenEmbedding:
         block size of the arena in which it begins at `first_value`.  `out`
         (tokens, width): fp32 or bf16, any row stride."""
         count, bytes_ = _tokens(tokens, device)
-        vocab, width, kind = _table(table, "table", device, _FLOATS + (torch.int8,))
+        vocab, width, kind = _table(table, "table", device, _FLOATS + _INT8)
         out_stride = _rows(out, "out", device, width, _FLOATS, count)
+        scales = 0
         if kind == 2:
             if table_scales is None or block_size < 0 or first_value < 0:
                 raise ValueError("an encoded table needs its scales, block size and place in the arena")
-            _require(table_scales, torch.float32, "table_scales", device)
             needed = 1 if block_size == 0 else (first_value + vocab * width + block_size - 1) // block_size
             if table_scales.numel() < needed:
                 raise ValueError(f"table_scales has {table_scales.numel()} values, needs {needed}")
+            scales = _vector(table_scales, "table_scales", device, table_scales.numel(), _FLOAT32)
         elif table_scales is not None:
             raise ValueError("a table that is not encoded has no scales")
-        if token_status is not None:
-            _require(token_status, torch.int32, "token_status", device)
         check("embedding_lookup", load().nntrain_embedding_lookup(
-            device, kind, table.data_ptr(), _ptr(table_scales), block_size, first_value, vocab, width, tokens.data_ptr(),
-            bytes_, count, padding_token, scale, _kind(out), out.data_ptr(), out_stride, _ptr(token_status),
+            device, kind, table.data_ptr(), scales, block_size, first_value, vocab, width, tokens.data_ptr(), bytes_, count,
+            padding_token, scale, _kind(out), out.data_ptr(), out_stride, _status(token_status, "token_status", device),
             _stream_on(device, stream)))
 
     @staticmethod
@@ -643,28 +670,26 @@ class TokenEmbedding:
         count, bytes_ = _tokens(tokens, device)
         vocab, width, kind = _table(table_gradient, "table_gradient", device, _FLOATS)
         stride = _rows(out_gradient, "out_gradient", device, width, _FLOATS, count)
-        if token_status is not None:
-            _require(token_status, torch.int32, "token_status", device)
-        workspace, workspace_bytes = _workspace("embedding_gradient", load().nntrain_embedding_gradient_workspace,
-                                                (count, vocab, width), device, workspace, stream)
+        workspace, workspace_bytes = _workspace("nntrain_embedding_gradient_workspace", (count, vocab, width), device,
+                                                workspace, stream)
         check("embedding_gradient", load().nntrain_embedding_gradient(
             device, _kind(out_gradient), out_gradient.data_ptr(), stride, tokens.data_ptr(), bytes_, count, padding_token,
-            scale, kind, table_gradient.data_ptr(), vocab, width, int(accumulate), _ptr(token_status), _ptr(workspace),
-            workspace_bytes, _stream_on(device, stream)))
+            scale, kind, table_gradient.data_ptr(), vocab, width, accumulate, _status(token_status, "token_status", device),
+            0 if workspace is None else workspace.data_ptr(), workspace_bytes, _stream_on(device, stream)))
 
 
 def _tokens(tokens: torch.Tensor, device: int) -> tuple[int, int]:
-    if tokens.dtype not in (torch.int32, torch.int64):
+    if tokens.dtype not in _INTEGERS:
         raise ValueError(f"tokens must be int32 or int64, got {tokens.dtype}")
-    _require(tokens, tokens.dtype, "tokens", device)
-    return tokens.numel(), tokens.element_size()
+    count = tokens.numel()
+    _vector(tokens, "tokens", device, count, _INTEGERS)
+    return count, 8 if tokens.dtype is torch.int64 else 4
 
 
 def _table(table: torch.Tensor, name: str, device: int, dtypes) -> tuple[int, int, int]:
     """(rows, width, kind) of a token table."""
-    _require(table, table.dtype, name, device)
-    if table.dtype not in dtypes:
-        raise ValueError(f"{name} has type {table.dtype}, expected one of {', '.join(map(str, dtypes))}")
-    if table.dim() != 2 or table.numel() == 0:
-        raise ValueError(f"{name} has shape {tuple(table.shape)}, expected (vocab, width)")
-    return table.shape[0], table.shape[1], 2 if table.dtype == torch.int8 else _kind(table)
+    _vector(table, name, device, table.numel(), dtypes)
+    shape = table.shape
+    if len(shape) != 2 or not shape[0] or not shape[1]:
+        raise ValueError(f"{name} has shape {tuple(shape)}, expected (vocab, width)")
+    return shape[0], shape[1], 2 if table.dtype is torch.int8 else _kind(table)
