@@ -42,25 +42,31 @@ struct RowSum {
     int turn;
 };
 
-// Sum / maximum over the CTA, the same value in every thread.  Two sets of
-// slots take turns, so one barrier per reduction is enough: a set is written
-// again only behind the barrier of the other one.
+template <bool kMaximum>
+__device__ __forceinline__ float combine(float a, float b) {
+    return kMaximum ? fmaxf(a, b) : __fadd_rn(a, b);
+}
+
+// Sum / maximum of values that are not negative (or any sum) over the CTA, the
+// same value in every thread.  Two sets of slots take turns, so one barrier per
+// reduction is enough: a set is written again only behind the barrier of the
+// other one.
 template <bool kMaximum>
 __device__ __forceinline__ float over_cta(float v, RowSum& s) {
     #pragma unroll
-    for (int offset = 16; offset > 0; offset >>= 1) {
-        const float other = __shfl_xor_sync(0xffffffffu, v, offset);
-        v = kMaximum ? fmaxf(v, other) : __fadd_rn(v, other);
-    }
+    for (int offset = 16; offset > 0; offset >>= 1) v = combine<kMaximum>(v, __shfl_xor_sync(0xffffffffu, v, offset));
     const int warps = blockDim.x >> 5;
     if (warps == 1) return v;
     float* slots = s.slots[s.turn];
     s.turn ^= 1;
-    if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) slots[threadIdx.x >> 5] = v;
     __syncthreads();
-    float total = slots[0];
-    for (int w = 1; w < warps; ++w) total = kMaximum ? fmaxf(total, slots[w]) : __fadd_rn(total, slots[w]);
-    return total;
+    // every warp adds the (at most 16) warps' values: a load and four shuffles
+    v = (lane & 15) < warps ? slots[lane & 15] : 0.0f;
+    #pragma unroll
+    for (int offset = 8; offset > 0; offset >>= 1) v = combine<kMaximum>(v, __shfl_xor_sync(0xffffffffu, v, offset));
+    return v;
 }
 
 // ---- loads and stores of a group -------------------------------------------------
@@ -123,12 +129,54 @@ __device__ __forceinline__ void load_row(const void* base, long long row, long l
     }
 }
 
-// Whether the next row is loaded ahead: where the raw groups of `inputs` rows are
-// few registers, so that they do not cost resident CTAs.
+// Rows on their way, in shared memory: every thread copies the groups that it
+// will read itself (cp.async, 16 bytes each) kStages - 1 rows ahead, so loads
+// cost no registers and a thread waits for its own copies only.  No stages for
+// rows with more than two 16-byte words a thread and input: those have enough
+// loads in flight by themselves.
 template <typename T, int kVec, int kGroups>
-__host__ __device__ constexpr bool loads_ahead(int inputs) {
-    return kVec == 8 && inputs * kGroups * 2 * static_cast<int>(sizeof(T)) <= 16;
+__host__ __device__ constexpr int row_stages() {
+    constexpr int kWords = kGroups * static_cast<int>(sizeof(T)) / 2;
+    return kVec == 1 || kWords > 2 ? 0 : (kWords == 1 ? 3 : 2);
 }
+
+__device__ __forceinline__ void copy_async16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<unsigned>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void close_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kOpen>
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(kOpen) : "memory"); }
+
+template <typename T, int kVec, int kGroups, int kInputs>
+struct RowRing {
+    static constexpr int kStages = row_stages<T, kVec, kGroups>();
+    static constexpr int kWords = static_cast<int>(sizeof(T)) / 2;      // 16-byte words of a group
+    static constexpr int kThreadBytes = kStages * kInputs * kGroups * kWords * 16;
+
+    uint4* words;                      // [stage][input][group][word][thread]
+
+    __device__ __forceinline__ uint4* at(int stage, int input, int group, int word) const {
+        return words + (((stage * kInputs + input) * kGroups + group) * kWords + word) * static_cast<int>(blockDim.x) + threadIdx.x;
+    }
+    __device__ __forceinline__ void copy(int stage, int input, const void* base, long long row, long long stride, int width) const {
+        const T* p = static_cast<const T*>(base) + row * stride + column_of<kVec, kGroups>(0);
+        #pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            if (column_of<kVec, kGroups>(g) >= width) continue;
+            #pragma unroll
+            for (int w = 0; w < kWords; ++w) copy_async16(at(stage, input, g, w), reinterpret_cast<const uint4*>(p + g * 32 * kVec) + w);
+        }
+    }
+    __device__ __forceinline__ void read(int stage, int input, Raw<T, kVec> (&raw)[kGroups]) const {
+        if constexpr (kVec == 8) {
+            #pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                #pragma unroll
+                for (int w = 0; w < kWords; ++w) raw[g].words[w] = *at(stage, input, g, w);
+            }
+        }
+    }
+};
 
 template <typename T>
 __device__ __forceinline__ float load_value(const T* p) {
@@ -200,13 +248,23 @@ struct ForwardArguments {
     long long rows, x_stride, residual_stride;
     int width, block, weight_kind, y_kind;
     bool weight_aligned;
-    float epsilon;
+    float epsilon, reciprocal_width;
 };
 
-__device__ __forceinline__ float inverse_of(float squares, int width, float epsilon, bool& bad) {
-    const float mean = __fdiv_rn(squares, static_cast<float>(width));
-    bad |= is_non_finite(mean);
-    return __frsqrt_rn(__fadd_rn(mean, epsilon));
+// 1 / sqrt(squares / width + epsilon).  The mean is a product with fl(1/width)
+// and the root the hardware's estimate (relative error below 2^-22) after one
+// Newton step, v + v/2 (1 - x v^2): three halves of a rounding off, and a few
+// instructions where the correctly rounded operations take some thirty, in every
+// warp of every row.
+__device__ __forceinline__ float inverse_of(float squares, float reciprocal_width, float epsilon, bool& bad) {
+    const float mean = __fmul_rn(squares, reciprocal_width);
+    const float x = __fadd_rn(mean, epsilon);
+    const float v = rsqrtf(x);
+    // for x of 0 or infinity the estimate is the answer, and the step would make it NaN
+    const float refined = __fmaf_rn(__fmul_rn(0.5f, v), __fmaf_rn(-__fmul_rn(x, v), v, 1.0f), v);
+    const float inverse = x > 0.0f && !is_non_finite(x) ? refined : v;
+    bad |= is_non_finite(mean) || is_non_finite(inverse);
+    return inverse;
 }
 
 template <int kVec>
@@ -250,19 +308,49 @@ rms_norm_forward_kernel(ForwardArguments a) {
             if (column < a.width) load_weights<kVec>(a.weight, a.weight_kind, a.weight_aligned, column, kept[kKeep ? g : 0]);
         }
     }
-    constexpr bool kAhead = loads_ahead<T, kVec, kGroups>(2);
+    extern __shared__ uint4 ring_words[];
+    using Ring = RowRing<T, kVec, kGroups, 2>;
+    const Ring ring{ring_words};
+    constexpr int kStages = Ring::kStages;
     Raw<T, kVec> x[kGroups], r[kGroups];
-    auto load = [&](long long row) {
-        load_row<T, kVec, kGroups>(a.x, row, a.x_stride, a.width, x);
-        if (a.residual != nullptr) load_row<T, kVec, kGroups>(a.residual, row, a.residual_stride, a.width, r);
+    auto copy = [&](long long row, int stage) {
+        if (row < a.rows) {
+            ring.copy(stage, 0, a.x, row, a.x_stride, a.width);
+            if (a.residual != nullptr) ring.copy(stage, 1, a.residual, row, a.residual_stride, a.width);
+        }
+        close_copies();                          // an empty one too: the waits count them
     };
+    // A y that is not finite has an h that is not (the mean shows it), a weight
+    // that is not (checked here, once) or overflows (its block's maximum shows
+    // it); where there is no maximum every y is looked at: y * 0 is 0 or NaN.
+    constexpr bool kCheckValues = kBlock < 0 || !kKeep;
     bool bad = false;
-    float not_finite = 0.0f;                     // NaN once a y is not finite: y * 0 is 0 or NaN
-    if (kAhead && blockIdx.x < a.rows) load(blockIdx.x);
+    float not_finite = 0.0f;
+    if (kKeep) {
+        #pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            #pragma unroll
+            for (int i = 0; i < kVec; ++i) bad |= is_non_finite(kept[kKeep ? g : 0][i]);
+        }
+    }
+    int stage = 0;
+    if constexpr (kStages > 0) {
+        #pragma unroll
+        for (int s = 0; s < kStages - 1; ++s) copy(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+    }
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const long long base = row * a.width;
         float h[kGroups][kVec];
-        if (!kAhead) load(row);
+        if constexpr (kStages > 0) {
+            copy(row + static_cast<long long>(kStages - 1) * gridDim.x, stage == 0 ? kStages - 1 : stage - 1);
+            wait_copies<kStages - 1>();
+            ring.read(stage, 0, x);
+            if (a.residual != nullptr) ring.read(stage, 1, r);
+            stage = stage == kStages - 1 ? 0 : stage + 1;
+        } else {
+            load_row<T, kVec, kGroups>(a.x, row, a.x_stride, a.width, x);
+            if (a.residual != nullptr) load_row<T, kVec, kGroups>(a.residual, row, a.residual_stride, a.width, r);
+        }
         #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
             const int column = column_of<kVec, kGroups>(g);
@@ -277,7 +365,6 @@ rms_norm_forward_kernel(ForwardArguments a) {
                 for (int i = 0; i < kVec; ++i) h[g][i] = __fadd_rn(h[g][i], v[i]);
             }
         }
-        if (kAhead && row + gridDim.x < a.rows) load(row + gridDim.x);
         float squares = 0.0f;
         #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
@@ -287,7 +374,7 @@ rms_norm_forward_kernel(ForwardArguments a) {
             #pragma unroll
             for (int i = 0; i < kVec; ++i) squares = __fmaf_rn(h[g][i], h[g][i], squares);
         }
-        const float inverse = inverse_of(over_cta<false>(squares, sums), a.width, a.epsilon, bad);
+        const float inverse = inverse_of(over_cta<false>(squares, sums), a.reciprocal_width, a.epsilon, bad);
         if (a.inverse_rms != nullptr && threadIdx.x == 0) a.inverse_rms[row] = inverse;
         float largest = 0.0f;
         #pragma unroll
@@ -298,13 +385,15 @@ rms_norm_forward_kernel(ForwardArguments a) {
             #pragma unroll
             for (int i = 0; i < kVec; ++i) {
                 h[g][i] = __fmul_rn(__fmul_rn(h[g][i], inverse), kKeep ? kept[kKeep ? g : 0][i] : w[i]);
-                not_finite = __fmaf_rn(h[g][i], 0.0f, not_finite);
+                if (kCheckValues) not_finite = __fmaf_rn(h[g][i], 0.0f, not_finite);
                 if (kBlock == 0) largest = fmaxf(largest, fabsf(h[g][i]));
             }
         }
         float row_scale = 1.0f;
         if constexpr (kBlock == 0) {
-            row_scale = scale_from_maximum_fast(over_cta<true>(largest, sums));
+            largest = over_cta<true>(largest, sums);
+            bad |= is_non_finite(largest);
+            row_scale = scale_from_maximum_fast(largest);
             if (threadIdx.x == 0) a.scales[row] = row_scale;
         }
         if constexpr (kVec == 1 && kBlock == 0) {
@@ -330,7 +419,9 @@ rms_norm_forward_kernel(ForwardArguments a) {
                 float maximum = 0.0f;
                 #pragma unroll
                 for (int i = 0; i < kVec; ++i) maximum = fmaxf(maximum, fabsf(h[g][i]));
-                const float scale = scale_from_maximum_fast(group_max<kLanes>(maximum));
+                maximum = group_max<kLanes>(maximum);
+                bad |= is_non_finite(maximum);
+                const float scale = scale_from_maximum_fast(maximum);
                 if (column < a.width) {
                     if (threadIdx.x % kLanes == 0) a.scales[(base + column) / kBlock] = scale;
                     encode_group<kVec>(h[g], scale, a.payload + base + column);
@@ -371,7 +462,7 @@ rms_norm_forward_loop_kernel(ForwardArguments a) {
             const float h = h_at(i);
             squares = __fmaf_rn(h, h, squares);
         }
-        const float inverse = inverse_of(over_cta<false>(squares, sums), a.width, a.epsilon, bad);
+        const float inverse = inverse_of(over_cta<false>(squares, sums), a.reciprocal_width, a.epsilon, bad);
         if (a.inverse_rms != nullptr && threadIdx.x == 0) a.inverse_rms[row] = inverse;
         auto y_of = [&](float h, int i) {
             return __fmul_rn(__fmul_rn(h, inverse), load_weight(a.weight, a.weight_kind, i));
@@ -420,6 +511,7 @@ struct BackwardArguments {
     long long rows, y_stride, residual_stride, h_stride;
     int width, weight_kind;
     bool weight_aligned;
+    float reciprocal_width;
 };
 
 template <typename T, int kVec, int kGroups>
@@ -437,21 +529,37 @@ rms_norm_backward_kernel(BackwardArguments a) {
             if (column < a.width) load_weights<kVec>(a.weight, a.weight_kind, a.weight_aligned, column, kept[kKeep ? g : 0]);
         }
     }
-    const float width = static_cast<float>(a.width);
-    constexpr bool kAhead = loads_ahead<T, kVec, kGroups>(3);
-    Raw<T, kVec> dy[kGroups], h[kGroups], r[kGroups];
-    float inverse_ahead = 0.0f;
-    auto load = [&](long long row) {
-        load_row<T, kVec, kGroups>(a.y_gradient, row, a.y_stride, a.width, dy);
-        load_row<T, kVec, kGroups>(a.h, row, a.h_stride, a.width, h);
-        if (kAhead && a.residual_gradient != nullptr)
-            load_row<T, kVec, kGroups>(a.residual_gradient, row, a.residual_stride, a.width, r);
-        inverse_ahead = a.inverse_rms[row];
+    extern __shared__ uint4 ring_words[];
+    using Ring = RowRing<T, kVec, kGroups, 3>;
+    const Ring ring{ring_words};
+    constexpr int kStages = Ring::kStages;
+    Raw<T, kVec> dy[kGroups], h[kGroups];
+    auto copy = [&](long long row, int stage) {
+        if (row < a.rows) {
+            ring.copy(stage, 0, a.y_gradient, row, a.y_stride, a.width);
+            ring.copy(stage, 1, a.h, row, a.h_stride, a.width);
+            if (a.residual_gradient != nullptr) ring.copy(stage, 2, a.residual_gradient, row, a.residual_stride, a.width);
+        }
+        close_copies();                          // an empty one too: the waits count them
     };
-    if (kAhead && blockIdx.x < a.rows) load(blockIdx.x);
+    int stage = 0;
+    float inverse_ahead = blockIdx.x < a.rows ? a.inverse_rms[blockIdx.x] : 0.0f;
+    if constexpr (kStages > 0) {
+        #pragma unroll
+        for (int s = 0; s < kStages - 1; ++s) copy(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+    }
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        if (!kAhead) load(row);
         const float inverse = inverse_ahead;
+        if (row + gridDim.x < a.rows) inverse_ahead = a.inverse_rms[row + gridDim.x];
+        if constexpr (kStages > 0) {
+            copy(row + static_cast<long long>(kStages - 1) * gridDim.x, stage == 0 ? kStages - 1 : stage - 1);
+            wait_copies<kStages - 1>();
+            ring.read(stage, 0, dy);
+            ring.read(stage, 1, h);
+        } else {
+            load_row<T, kVec, kGroups>(a.y_gradient, row, a.y_stride, a.width, dy);
+            load_row<T, kVec, kGroups>(a.h, row, a.h_stride, a.width, h);
+        }
         float d[kGroups][kVec], n[kGroups][kVec];
         float along = 0.0f;
         #pragma unroll
@@ -473,20 +581,20 @@ rms_norm_backward_kernel(BackwardArguments a) {
                 along = __fmaf_rn(d[g][i], n[g][i], along);
             }
         }
+        const float mean = __fmul_rn(over_cta<false>(along, sums), a.reciprocal_width);
         Raw<T, kVec> added[kGroups];
-        if (kAhead) {
-            #pragma unroll
-            for (int g = 0; g < kGroups; ++g) added[g] = r[g];
-            if (row + gridDim.x < a.rows) load(row + gridDim.x);
+        if constexpr (kStages > 0) {
+            if (a.residual_gradient != nullptr) ring.read(stage, 2, added);
+            stage = stage == kStages - 1 ? 0 : stage + 1;
         }
-        const float mean = __fdiv_rn(over_cta<false>(along, sums), width);
         #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
             const int column = column_of<kVec, kGroups>(g);
             if (column >= a.width) continue;
             float v[kVec] = {};
             if (a.residual_gradient != nullptr) {
-                if (!kAhead) load_raw<T, kVec>(static_cast<const T*>(a.residual_gradient) + row * a.residual_stride + column, added[g]);
+                if constexpr (kStages == 0)
+                    load_raw<T, kVec>(static_cast<const T*>(a.residual_gradient) + row * a.residual_stride + column, added[g]);
                 unpack<T, kVec>(added[g], v);
             }
             #pragma unroll
@@ -523,7 +631,7 @@ rms_norm_backward_loop_kernel(BackwardArguments a) {
             partial[i] = __fmaf_rn(d, n, partial[i]);
             along = __fmaf_rn(__fmul_rn(d, load_weight(a.weight, a.weight_kind, i)), n, along);
         }
-        const float mean = __fdiv_rn(over_cta<false>(along, sums), static_cast<float>(a.width));
+        const float mean = __fmul_rn(over_cta<false>(along, sums), a.reciprocal_width);
         for (int i = threadIdx.x; i < a.width; i += kLoopThreads) {
             const float g = __fmul_rn(load_value(dy + i), load_weight(a.weight, a.weight_kind, i));
             const float n = __fmul_rn(load_value(h + i), inverse);
@@ -564,14 +672,15 @@ rms_norm_join_kernel(const float* partials, int count, int width, void* weight_g
 
 // ---- launch shapes ---------------------------------------------------------------
 
-// One resident wave of kKernel with `threads` threads.
+// One resident wave of kKernel with `threads` threads and the shared memory that
+// goes with them.
 template <auto kKernel>
-int resident_grid(int threads, long long rows) {
+int resident_grid(int threads, int shared, long long rows) {
     static std::atomic<int> known[kRowThreads / 32 + 1];
     std::atomic<int>& slot = known[threads / 32];
     int fit = slot.load(std::memory_order_relaxed);
     if (fit == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kKernel, threads, 0) != cudaSuccess || fit < 1) fit = 1;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kKernel, threads, shared) != cudaSuccess || fit < 1) fit = 1;
         slot.store(fit, std::memory_order_relaxed);
     }
     return grid_for(rows, fit);
@@ -581,25 +690,35 @@ struct RowShape {
     int groups, threads;               // groups 0: the row does not fit registers
 };
 
-// Threads and groups per thread for a row of `units` groups of 8 values: the
-// fewest groups that keep a row within 256 threads, so several rows share an SM
-// and their barriers overlap; few rows (fewer than SMs) get more threads each.
 int threads_for(int units, int groups) { return ((units + groups - 1) / groups + 31) / 32 * 32; }
 
-RowShape row_shape(int units, long long rows) {
-    const int want = rows < sm_count() ? kRowThreads : 256;
+// Threads and groups per thread for a row of `units` groups of 8 values: the
+// fewest groups that keep a row within 256 threads, so several rows share an SM
+// and their barriers overlap.  (16384 x 1536 bf16: 45 us with 192 threads, 47 us
+// with 96, 61 us with 64.)
+RowShape row_shape(int units) {
     for (int groups = 1; groups <= 4; groups *= 2) {
         const int threads = threads_for(units, groups);
-        if (threads <= want || (groups == 4 && threads <= kRowThreads)) return {groups, threads};
+        if (threads <= 256 || (groups == 4 && threads <= kRowThreads)) return {groups, threads};
     }
     return {0, 0};
+}
+
+// Rows that are staged have at most 256 threads, so at most 48 KB in flight: with
+// the reduction's slots a little more than a launch may ask for by itself.
+template <auto kKernel>
+cudaError_t allow_shared(int shared) {
+    return shared < (40 << 10) ? cudaSuccess
+                               : cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
 }
 
 template <typename T, int kVec, int kGroups, int kBlock>
 cudaError_t launch_forward(const ForwardArguments& a, int threads, cudaStream_t stream) {
     constexpr auto kKernel = rms_norm_forward_kernel<T, kVec, kGroups, kBlock>;
-    const int grid = resident_grid<kKernel>(threads, a.rows);
-    kKernel<<<grid, threads, 0, stream>>>(a);
+    const int shared = threads * RowRing<T, kVec, kGroups, 2>::kThreadBytes;
+    const cudaError_t e = allow_shared<kKernel>(shared);
+    if (e != cudaSuccess) return e;
+    kKernel<<<resident_grid<kKernel>(threads, shared, a.rows), threads, shared, stream>>>(a);
     return cudaPeekAtLastError();
 }
 
@@ -619,32 +738,37 @@ template <typename T>
 cudaError_t run_forward(const ForwardArguments& a, bool vector_ok, cudaStream_t stream) {
     const bool whole = a.payload == nullptr || a.block == a.width;
     if (vector_ok && (whole || a.block == 32 || a.block == 64 || a.block == 128)) {
-        const RowShape s = row_shape(a.width / 8, a.rows);
+        const RowShape s = row_shape(a.width / 8);
         if (s.groups == 1) return forward_by_block<T, 8, 1>(a, s.threads, stream);
         if (s.groups == 2) return forward_by_block<T, 8, 2>(a, s.threads, stream);
         if (s.groups == 4) return forward_by_block<T, 8, 4>(a, s.threads, stream);
     } else if (whole || a.block == 32) {
-        if (a.width <= 4 * kRowThreads) return forward_by_block<T, 1, 4>(a, threads_for(a.width, 4), stream);
+        // 16 values a thread past one warp's: the barriers and the row's own arithmetic are shared by fewer warps
+        // (3001 x 771 fp32: 16.4 us with 4 or 8 values, 12.3 us with 16)
+        if (a.width <= 512) return forward_by_block<T, 1, 4>(a, threads_for(a.width, 4), stream);
         if (a.width <= 16 * kRowThreads) return forward_by_block<T, 1, 16>(a, threads_for(a.width, 16), stream);
     }
     constexpr auto kKernel = rms_norm_forward_loop_kernel<T>;
-    kKernel<<<resident_grid<kKernel>(kLoopThreads, a.rows), kLoopThreads, 0, stream>>>(a);
+    kKernel<<<resident_grid<kKernel>(kLoopThreads, 0, a.rows), kLoopThreads, 0, stream>>>(a);
     return cudaPeekAtLastError();
 }
 
 template <typename T, int kVec, int kGroups>
 cudaError_t launch_backward(const BackwardArguments& a, int threads, int& grid, cudaStream_t stream) {
     constexpr auto kKernel = rms_norm_backward_kernel<T, kVec, kGroups>;
-    grid = resident_grid<kKernel>(threads, a.rows);
+    const int shared = threads * RowRing<T, kVec, kGroups, 3>::kThreadBytes;
+    const cudaError_t e = allow_shared<kKernel>(shared);
+    if (e != cudaSuccess) return e;
+    grid = resident_grid<kKernel>(threads, shared, a.rows);
     if (grid > kMostPartials) grid = kMostPartials;
-    kKernel<<<grid, threads, 0, stream>>>(a);
+    kKernel<<<grid, threads, shared, stream>>>(a);
     return cudaPeekAtLastError();
 }
 
 template <typename T>
 cudaError_t run_backward(const BackwardArguments& a, bool vector_ok, int& grid, cudaStream_t stream) {
     if (vector_ok) {
-        const RowShape s = row_shape(a.width / 8, a.rows);
+        const RowShape s = row_shape(a.width / 8);
         if (s.groups == 1) return launch_backward<T, 8, 1>(a, s.threads, grid, stream);
         if (s.groups == 2) return launch_backward<T, 8, 2>(a, s.threads, grid, stream);
         if (s.groups == 4) return launch_backward<T, 8, 4>(a, s.threads, grid, stream);
@@ -653,7 +777,7 @@ cudaError_t run_backward(const BackwardArguments& a, bool vector_ok, int& grid, 
         if (a.width <= 16 * kRowThreads) return launch_backward<T, 1, 16>(a, threads_for(a.width, 16), grid, stream);
     }
     constexpr auto kKernel = rms_norm_backward_loop_kernel<T>;
-    grid = resident_grid<kKernel>(kLoopThreads, a.rows);
+    grid = resident_grid<kKernel>(kLoopThreads, 0, a.rows);
     if (grid > kMostPartials) grid = kMostPartials;
     kKernel<<<grid, kLoopThreads, 0, stream>>>(a);
     return cudaPeekAtLastError();
@@ -688,7 +812,7 @@ int forward(int device, int kind, const void* x, long long x_stride, const void*
     const DeviceScope scope(device);
     if (scope.status() != cudaSuccess) return scope.status();
     const ForwardArguments a{x, residual, weight, residual_out, y, payload, scales, inverse_rms, finite_status,
-                             rows, x_stride, residual_stride, width, block, weight_kind, y_kind, aligned_for(weight, 16), epsilon};
+                             rows, x_stride, residual_stride, width, block, weight_kind, y_kind, aligned_for(weight, 16), epsilon, 1.0f / static_cast<float>(width)};
     const bool vector_ok = width % 8 == 0 && rows_aligned(x, kind, x_stride) &&
                            (!residual || rows_aligned(residual, kind, residual_stride)) &&
                            aligned_for(residual_out, 16) && aligned_for(y, 16) && aligned_for(payload, 8);
@@ -715,7 +839,7 @@ int backward(int device, int kind, const void* y_gradient, long long y_stride, c
     cudaError_t e = cudaSuccess;
     if (rows > 0) {
         const BackwardArguments a{y_gradient, residual_gradient, h, weight, inverse_rms, x_gradient,
-                                  static_cast<float*>(workspace), rows, y_stride, residual_stride, h_stride, width, weight_kind, aligned_for(weight, 16)};
+                                  static_cast<float*>(workspace), rows, y_stride, residual_stride, h_stride, width, weight_kind, aligned_for(weight, 16), 1.0f / static_cast<float>(width)};
         const bool vector_ok = width % 8 == 0 && rows_aligned(y_gradient, kind, y_stride) && rows_aligned(h, kind, h_stride) &&
                                (!residual_gradient || rows_aligned(residual_gradient, kind, residual_stride)) &&
                                aligned_for(x_gradient, 16);

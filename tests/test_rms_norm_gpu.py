@@ -5,10 +5,11 @@ step of the output's type (0 where it is fp32 and counted already):
   squares  a sum of `width` non-negative products; no value passes more than
            d = terms of a thread + 5 butterfly steps + 16 warps additions:
            (d + 2) e, the 2 for h = fl(x + r) squared
-  i        mean and + epsilon add 2 e, the root halves, its own rounding adds e
+  i        the mean, a product with fl(1/width), adds 2 e, + epsilon e; the root
+           halves; its Newton step is 3/2 e off
   y        i's, and h, two products: 3 e more
   code     |code - y/scale| <= 1/2 + 127 (2 y's + 2 e), for y and scale both
-  dx       i (g - n c) + r with c = mean(g n): (d + 4) e of mean|g n| in c, a
+  dx       i (g - n c) + r with c = mean(g n): (d + 5) e of mean|g n| in c, a
            step for each of g, n, their product, the sums and the result
   dw       rows / 148 terms a block, 37 + 5 in the join, 2 e for the product"""
 import numpy as np
@@ -31,7 +32,7 @@ def depth(width):
 
 
 def tolerance_i(width):
-    return ((depth(width) + 4) / 2 + 1) * E
+    return ((depth(width) + 5) / 2 + 1.5) * E
 
 
 def f64(t):
