@@ -692,12 +692,16 @@ struct RowShape {
 
 int threads_for(int units, int groups) { return ((units + groups - 1) / groups + 31) / 32 * 32; }
 
-// Threads and groups per thread for a row of `units` groups of 8 values: the
-// fewest groups that keep a row within 256 threads, so several rows share an SM
-// and their barriers overlap.  (16384 x 1536 bf16: 45 us with 192 threads, 47 us
-// with 96, 61 us with 64.)
-RowShape row_shape(int units) {
-    for (int groups = 1; groups <= 4; groups *= 2) {
+// Threads and groups per thread for a row of `units` groups of 8 values.  32
+// bytes of an input a thread (two groups of bf16, one of fp32) where there are
+// rows for all SMs, so that few warps share a row's barriers and its own
+// arithmetic (16384 x 1536 bf16: 43 us with 96 threads, 45 us with 192, 54 us
+// with 64; its gradient 69, 78 and 100 us for twice the rows), more where the row
+// is longer than 256 threads then.
+template <typename T>
+RowShape row_shape(int units, long long rows) {
+    const bool wide = sizeof(T) == 2 && units > 64 && rows >= sm_count();
+    for (int groups = wide ? 2 : 1; groups <= 4; groups *= 2) {
         const int threads = threads_for(units, groups);
         if (threads <= 256 || (groups == 4 && threads <= kRowThreads)) return {groups, threads};
     }
@@ -738,7 +742,7 @@ template <typename T>
 cudaError_t run_forward(const ForwardArguments& a, bool vector_ok, cudaStream_t stream) {
     const bool whole = a.payload == nullptr || a.block == a.width;
     if (vector_ok && (whole || a.block == 32 || a.block == 64 || a.block == 128)) {
-        const RowShape s = row_shape(a.width / 8);
+        const RowShape s = row_shape<T>(a.width / 8, a.rows);
         if (s.groups == 1) return forward_by_block<T, 8, 1>(a, s.threads, stream);
         if (s.groups == 2) return forward_by_block<T, 8, 2>(a, s.threads, stream);
         if (s.groups == 4) return forward_by_block<T, 8, 4>(a, s.threads, stream);
@@ -768,7 +772,7 @@ cudaError_t launch_backward(const BackwardArguments& a, int threads, int& grid, 
 template <typename T>
 cudaError_t run_backward(const BackwardArguments& a, bool vector_ok, int& grid, cudaStream_t stream) {
     if (vector_ok) {
-        const RowShape s = row_shape(a.width / 8);
+        const RowShape s = row_shape<T>(a.width / 8, a.rows);
         if (s.groups == 1) return launch_backward<T, 8, 1>(a, s.threads, grid, stream);
         if (s.groups == 2) return launch_backward<T, 8, 2>(a, s.threads, grid, stream);
         if (s.groups == 4) return launch_backward<T, 8, 4>(a, s.threads, grid, stream);
