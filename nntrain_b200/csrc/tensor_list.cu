@@ -35,6 +35,7 @@ namespace {
 enum TensorKind : int { kKindF32 = 0, kKindBf16 = 1, kKindBfp8 = 2 };
 
 constexpr int kUnroll = 4;              // 128-bit loads in flight per thread
+constexpr int kShiftedUnroll = 2;       // of two loads each
 constexpr int kFinishThreads = 1024;
 
 // A chunk is the same number of bytes for every kind: chunk_values fp32 values,
@@ -131,29 +132,59 @@ __device__ __forceinline__ double scale_square(float scale) {
     return square_of(scale);
 }
 
+// Number of the block that value `start + i` is in, for i of a chunk: one 64-bit
+// division a chunk, and a shift or a 32-bit one a value.
+struct BlockIndex {
+    long long first;                    // block of value `start`
+    unsigned offset, block;             // start's place in it, block size (0: one block)
+    int shift;                          // block = 1 << shift, or < 0
+
+    __device__ __forceinline__ BlockIndex(long long start, int block_size, bool one_block) {
+        block = one_block ? 0u : static_cast<unsigned>(block_size);
+        first = one_block ? 0 : start / block_size;
+        offset = one_block ? 0u : static_cast<unsigned>(start - first * block_size);
+        shift = one_block || (block & (block - 1u)) != 0 ? -1 : 31 - __clz(static_cast<int>(block));
+    }
+    __device__ __forceinline__ long long at(int i) const {
+        if (block == 0) return 0;
+        const unsigned place = offset + static_cast<unsigned>(i);
+        return first + (shift >= 0 ? place >> shift : place / block);
+    }
+};
+
+__device__ __forceinline__ int word_squares(const uint4& w) {
+    int sum = __dp4a(static_cast<int>(w.x), static_cast<int>(w.x), 0);
+    sum = __dp4a(static_cast<int>(w.y), static_cast<int>(w.y), sum);
+    sum = __dp4a(static_cast<int>(w.z), static_cast<int>(w.z), sum);
+    return __dp4a(static_cast<int>(w.w), static_cast<int>(w.w), sum);
+}
+
 // Codes [start, start + n) of a payload whose blocks of `block` values begin at
 // its first value.  A 16-byte word lies inside one block when block % 16 == 0
 // (or there is one block only) and the payload is 16-byte aligned; chunks start
 // at multiples of 4096 values.  Other layouts go value by value.
 __device__ double chunk_squares_bfp8(const signed char* payload, const float* scales, long long start, int n,
-                                     long long block, bool one_block) {
-    double a = 0.0;
-    const bool vector_ok = (reinterpret_cast<std::uintptr_t>(payload) & 15u) == 0 && (one_block || block % 16 == 0);
+                                     int block_size, bool one_block) {
+    const BlockIndex index(start, block_size, one_block);
+    const bool vector_ok = (reinterpret_cast<std::uintptr_t>(payload) & 15u) == 0 && (one_block || block_size % 16 == 0);
     const int vectors = vector_ok ? n >> 4 : 0;
     const uint4* body = reinterpret_cast<const uint4*>(payload + start);
-    for (int i = threadIdx.x; i < vectors; i += kThreads) {
-        const uint4 w = __ldg(body + i);
-        const float scale = __ldg(scales + (one_block ? 0 : (start + i * 16ll) / block));
-        int sum = __dp4a(static_cast<int>(w.x), static_cast<int>(w.x), 0);
-        sum = __dp4a(static_cast<int>(w.y), static_cast<int>(w.y), sum);
-        sum = __dp4a(static_cast<int>(w.z), static_cast<int>(w.z), sum);
-        sum = __dp4a(static_cast<int>(w.w), static_cast<int>(w.w), sum);
-        a += scale_square(scale) * static_cast<double>(sum);
+    double a = 0.0;
+    for (int i = threadIdx.x; i < vectors; i += kUnroll * kThreads) {
+        uint4 w[kUnroll];
+        float scale[kUnroll];
+        #pragma unroll
+        for (int j = 0; j < kUnroll; ++j) {
+            const int at = i + j * kThreads;
+            w[j] = at < vectors ? __ldg(body + at) : make_uint4(0, 0, 0, 0);
+            scale[j] = at < vectors ? __ldg(scales + index.at(at * 16)) : 1.0f;
+        }
+        #pragma unroll
+        for (int j = 0; j < kUnroll; ++j) a += scale_square(scale[j]) * static_cast<double>(word_squares(w[j]));
     }
     for (int i = vectors * 16 + threadIdx.x; i < n; i += kThreads) {
         const int code = payload[start + i];
-        const float scale = __ldg(scales + (one_block ? 0 : (start + i) / block));
-        a += scale_square(scale) * static_cast<double>(code * code);
+        a += scale_square(__ldg(scales + index.at(i))) * static_cast<double>(code * code);
     }
     return a;
 }
@@ -334,10 +365,10 @@ __device__ void clip_chunk(const T* source, T* destination, long long length, lo
         return reinterpret_cast<std::uintptr_t>(in + i) >= reinterpret_cast<std::uintptr_t>(first) &&
                reinterpret_cast<std::uintptr_t>(in + i + 2) <= reinterpret_cast<std::uintptr_t>(last);
     };
-    for (int i = threadIdx.x; i < words; i += kUnroll * kThreads) {
-        uint4 a[kUnroll], b[kUnroll];
+    for (int i = threadIdx.x; i < words; i += kShiftedUnroll * kThreads) {
+        uint4 a[kShiftedUnroll], b[kShiftedUnroll];
         #pragma unroll
-        for (int j = 0; j < kUnroll; ++j) {
+        for (int j = 0; j < kShiftedUnroll; ++j) {
             const int w = i + j * kThreads;
             if (w < words && inside(w)) {
                 a[j] = __ldg(in + w);
@@ -345,7 +376,7 @@ __device__ void clip_chunk(const T* source, T* destination, long long length, lo
             }
         }
         #pragma unroll
-        for (int j = 0; j < kUnroll; ++j) {
+        for (int j = 0; j < kShiftedUnroll; ++j) {
             const int w = i + j * kThreads;
             if (w >= words) continue;
             if (inside(w)) {
