@@ -109,10 +109,10 @@ embedding_lookup_kernel(LookupArguments a) {
     const int first = static_cast<int>(blockIdx.y) * kLookupColumns;
     const int here = static_cast<int>(a.count - position < kTokens ? a.count - position : kTokens);
     bool bad = false;
-    const long long mine = lane < here ? a.tokens.at(position + lane, bad) : -1;
+    const int mine = lane < here ? static_cast<int>(a.tokens.at(position + lane, bad)) : -1;
     if (bad && a.status != nullptr) atomicExch(a.status, 1);
     T* out = static_cast<T*>(a.out) + position * a.out_stride;
-    long long token[kTokens];
+    int token[kTokens];                          // (a row is below 2^31)
     #pragma unroll
     for (int t = 0; t < kTokens; ++t) token[t] = __shfl_sync(0xffffffffu, mine, t);
     if constexpr (kVector) {
@@ -124,7 +124,7 @@ embedding_lookup_kernel(LookupArguments a) {
         #pragma unroll
         for (int t = 0; t < kTokens; ++t) {
             if (token[t] < 0) continue;
-            const long long at = token[t] * a.width + column;
+            const long long at = static_cast<long long>(token[t]) * a.width + column;
             if constexpr (kTable == kTableBfp8) {
                 const uint2 x = __ldg(reinterpret_cast<const uint2*>(static_cast<const signed char*>(a.table) + at));
                 raw[t][0] = x.x; raw[t][1] = x.y;
@@ -160,7 +160,7 @@ embedding_lookup_kernel(LookupArguments a) {
         #pragma unroll
         for (int t = 0; t < kTokens; ++t) {
             if (t >= here) break;
-            const long long row = token[t] * a.width;
+            const long long row = static_cast<long long>(token[t]) * a.width;
             #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int column = first + i * 32 + lane;
@@ -637,20 +637,30 @@ __device__ unsigned last_chunk_of(const RowsArguments& a, unsigned key, unsigned
 template <int kValues, bool kVector>
 __device__ __forceinline__ void add_partials(const RowsArguments& a, unsigned begin, unsigned end, unsigned from, unsigned to,
                                              int first, int lane, float (&sum)[kValues]) {
-    #pragma unroll 4
-    for (unsigned p = from; p < to; ++p) {
-        const float* partial = (begin + p == end ? a.heads : a.tails) + static_cast<long long>(begin + p) * a.width;
+    constexpr int kBatch = 4;                    // partials whose loads are in flight together
+    for (unsigned p = from; p < to; p += kBatch) {
+        float values[kBatch][kValues];
         #pragma unroll
-        for (int i = 0; i < kValues; i += kVector ? 4 : 1) {
-            const int column = lane_column<kValues, kVector>(first, lane, i);
-            if (column >= a.width) continue;
-            if constexpr (kVector) {
-                const float4 x = load_f4(partial + column);
-                sum[i] = __fadd_rn(sum[i], x.x); sum[i + 1] = __fadd_rn(sum[i + 1], x.y);
-                sum[i + 2] = __fadd_rn(sum[i + 2], x.z); sum[i + 3] = __fadd_rn(sum[i + 3], x.w);
-            } else {
-                sum[i] = __fadd_rn(sum[i], partial[column]);
+        for (int b = 0; b < kBatch; ++b) {
+            const unsigned at = begin + p + b;
+            const float* partial = (at == end ? a.heads : a.tails) + static_cast<long long>(at) * a.width;
+            #pragma unroll
+            for (int i = 0; i < kValues; i += kVector ? 4 : 1) {
+                const int column = lane_column<kValues, kVector>(first, lane, i);
+                const bool here = p + b < to && column < a.width;
+                if constexpr (kVector) {
+                    const float4 x = here ? load_f4(partial + column) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    values[b][i] = x.x; values[b][i + 1] = x.y; values[b][i + 2] = x.z; values[b][i + 3] = x.w;
+                } else {
+                    values[b][i] = here ? partial[column] : 0.0f;
+                }
             }
+        }
+        #pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            if (p + b >= to) break;
+            #pragma unroll
+            for (int i = 0; i < kValues; ++i) sum[i] = __fadd_rn(sum[i], values[b][i]);
         }
     }
 }
