@@ -303,9 +303,11 @@ int nntrain_gradient_clip_apply(int device, int kind, void* values, long long co
 
 /* ABI minor 36.  Host only: cuts a list into the chunks its kernels work on.
  * Fills tensors[i].first_chunk and, when chunk_map is not null, 2 words per
- * chunk (tensor, index in the tensor); chunk_values is the length of a chunk.
- * Call it with a null chunk_map for the count, then with room for `capacity`
- * chunks; copy table and map to the device and use them for as long as
+ * chunk (tensor, index in the tensor); chunk_values is the length of a chunk of
+ * fp32 values (bf16: twice, BFP8: four times as long).  Call it with a null
+ * chunk_map for the count, then with room for `capacity` chunks.  The first call
+ * refuses a list in which what the clip writes for one tensor is read or written
+ * for another one (a tensor twice, a destination over a neighbour); copy table and map to the device and use them for as long as
  * addresses and lengths stay what they are. */
 int nntrain_gradient_list_plan(nntrain_gradient_tensor* tensors, int count, int* chunk_map,
                                long long capacity, long long* chunk_count, int* chunk_values);
@@ -349,7 +351,8 @@ int nntrain_optimizer_adamw_bfp8_gradient(
 
 /* h = x + residual (residual optional), i = 1 / sqrt(mean(h^2) + epsilon),
  * y = h * i * weight; fp32 arithmetic.  residual_out (optional, with a
- * residual): h, may be x or residual itself when that is contiguous.
+ * residual): h; it or y, of x's type, may be x or residual itself when that is
+ * contiguous.
  * inverse_rms (optional): i per row.  payload, scales (optional): y in the
  * codec's flat layout, so block_size (0 = one scale a row) has to divide width;
  * the codec's rules for values that are not finite hold.  y (at least one of y

@@ -29,6 +29,9 @@
 
 #include "nntrain_grad_abi.h"
 
+#include <algorithm>
+#include <vector>
+
 namespace ngb {
 namespace {
 
@@ -460,6 +463,50 @@ bool valid_tensor(const nntrain_gradient_tensor& t) {
            aligned_for(t.destination, t.kind == kKindBfp8 ? 4 : bytes);
 }
 
+struct Range {
+    std::uintptr_t begin, end;
+    int tensor;
+};
+
+// Whether what the clip writes for one tensor is read or written for another
+// one (the same tensor twice, a destination over a neighbour): chunks run in any
+// order, so such a list has no defined result.
+bool overlapping(const nntrain_gradient_tensor* tensors, int count) {
+    std::vector<Range> written, read;
+    for (int i = 0; i < count; ++i) {
+        const nntrain_gradient_tensor& t = tensors[i];
+        if (t.length == 0) continue;
+        const auto range = [&](const void* p, long long bytes) {
+            const std::uintptr_t at = reinterpret_cast<std::uintptr_t>(p);
+            return Range{at, at + static_cast<std::uintptr_t>(bytes), i};
+        };
+        if (t.kind == kKindBfp8) {
+            const long long blocks = t.block_size == 0 || t.block_size >= t.length ? 1 : (t.length + t.block_size - 1) / t.block_size;
+            read.push_back(range(t.values, t.length));
+            read.push_back(range(t.scales, blocks * 4));
+            written.push_back(range(t.destination != nullptr ? t.destination : t.scales, blocks * 4));
+        } else {
+            const long long bytes = t.length * (t.kind == kKindF32 ? 4 : 2);
+            read.push_back(range(t.values, bytes));
+            written.push_back(range(t.destination != nullptr ? t.destination : t.values, bytes));
+        }
+    }
+    const auto by_begin = [](const Range& a, const Range& b) { return a.begin < b.begin; };
+    std::sort(written.begin(), written.end(), by_begin);
+    for (size_t i = 1; i < written.size(); ++i)
+        if (written[i].begin < written[i - 1].end) return true;
+    for (const Range& r : read) {
+        // written ranges are apart: those that meet r are next to where it begins
+        auto w = std::upper_bound(written.begin(), written.end(), r, by_begin);
+        if (w != written.begin()) --w;
+        for (; w != written.end() && w->begin < r.end; ++w) {
+            const bool itself = w->tensor == r.tensor && w->begin == r.begin && w->end == r.end;
+            if (w->end > r.begin && !itself) return true;
+        }
+    }
+    return false;
+}
+
 int plan_list(nntrain_gradient_tensor* tensors, int count, int* chunk_map, long long capacity,
               long long* chunk_count, int* chunk_values) {
     if (!tensors || count <= 0 || !chunk_count || !chunk_values || capacity < 0)
@@ -469,6 +516,7 @@ int plan_list(nntrain_gradient_tensor* tensors, int count, int* chunk_map, long 
         if (!valid_tensor(tensors[i]) || tensors[i].length > (1ll << 46) - total) return static_cast<int>(cudaErrorInvalidValue);
         total += tensors[i].length >> tensors[i].kind;
     }
+    if (chunk_map == nullptr && overlapping(tensors, count)) return static_cast<int>(cudaErrorInvalidValue);
     long long size = (total / 2048 + kChunkLeast - 1) / kChunkLeast * kChunkLeast;
     size = size < kChunkLeast ? kChunkLeast : (size > kChunkMost ? kChunkMost : size);
     long long chunks = 0;
@@ -530,7 +578,13 @@ using namespace ngb;
 
 NNTRAIN_EXPORT int nntrain_gradient_list_plan(nntrain_gradient_tensor* tensors, int count, int* chunk_map,
                                               long long capacity, long long* chunk_count, int* chunk_values) {
-    return complete(kOpTensorList, -1, plan_list(tensors, count, chunk_map, capacity, chunk_count, chunk_values));
+    int status;
+    try {
+        status = plan_list(tensors, count, chunk_map, capacity, chunk_count, chunk_values);
+    } catch (...) {                      // the ranges are sorted in host memory
+        status = static_cast<int>(cudaErrorMemoryAllocation);
+    }
+    return complete(kOpTensorList, -1, status);
 }
 
 NNTRAIN_EXPORT int nntrain_gradient_list_clip(int device, const nntrain_gradient_tensor* tensors, int count,

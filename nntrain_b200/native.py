@@ -425,8 +425,10 @@ class GradientTensorList:
     """The gradient tensors of a model as one table on the device: fp32, bf16 and
     BFP8 (payload, with its scales and block size) tensors of any length and
     place, each with an optional destination for its clipped values (BFP8: its
-    clipped scales); without one it is clipped in place.  Build it once for
-    leaves that stay where they are; it holds on to the tensors."""
+    clipped scales); without one it is clipped in place.  What is written for one
+    tensor may not be read or written for another.  Build it once for leaves that
+    stay where they are; it holds on to the tensors, and a recorded graph needs
+    it to live as long as itself."""
 
     _TENSOR = np.dtype([("values", np.uint64), ("scales", np.uint64), ("destination", np.uint64),
                         ("length", np.int64), ("first_chunk", np.int64), ("kind", np.int32), ("block_size", np.int32)])
@@ -459,14 +461,15 @@ class GradientTensorList:
                     raise ValueError(f"destination of tensor {i} must have its type")
                 if to.numel() != source.numel():
                     raise ValueError(f"destination of tensor {i} must have its length")
-                apart = abs(to.data_ptr() - source.data_ptr())
-                if 0 < apart < source.numel() * source.element_size():
-                    raise ValueError(f"destination of tensor {i} overlaps it")
             table[i] = (t.data_ptr(), _ptr(s) if encoded else 0, _ptr(to), t.numel(), 0,
                         2 if encoded else _kind(t), block if encoded else 0)
         chunks, values = ctypes.c_longlong(), ctypes.c_int()
         plan = load().nntrain_gradient_list_plan
-        check("gradient_list_plan", plan(table.ctypes.data, count, None, 0, ctypes.addressof(chunks), ctypes.addressof(values)))
+        status = plan(table.ctypes.data, count, None, 0, ctypes.addressof(chunks), ctypes.addressof(values))
+        if status == 1:                       # types, lengths and addresses were checked above
+            raise ValueError("tensors and destinations of a gradient list must not overlap: what is written for one tensor "
+                             "may not be read or written for another")
+        check("gradient_list_plan", status)
         chunk_map = np.zeros((max(chunks.value, 1), 2), dtype=np.int32)
         check("gradient_list_plan", plan(table.ctypes.data, count, chunk_map.ctypes.data, chunks.value,
                                          ctypes.addressof(chunks), ctypes.addressof(values)))
@@ -564,7 +567,8 @@ class RmsNorm:
         `payload` and `scales`: y encoded, `block_size` values to a scale (a divisor
         of the width; 0 = one scale a row).  `y` (fp32 or bf16): y itself, or with a
         payload the values that the codes stand for.  `residual_out`: h, in x's
-        type (x or residual itself is allowed); `inverse_rms`: i for the gradient."""
+        type; `inverse_rms`: i for the gradient.  residual_out, or y in x's type,
+        may be x or residual itself."""
         if x.dim() != 2:
             raise ValueError(f"x has shape {tuple(x.shape)}, expected (rows, width)")
         rows, width = x.shape

@@ -164,6 +164,28 @@ def test_the_sum_may_take_the_place_of_an_input(cuda, width, block):
         assert all(torch.equal(p, q) for p, q in zip(results[0], other))
 
 
+@pytest.mark.parametrize("width", (1536, 771, 16416, 8193))
+@pytest.mark.parametrize("block", (None, 0, 32))
+def test_y_may_take_the_place_of_x(cuda, width, block):
+    if block and width % block:
+        block = 0
+    rows = 700                                        # some CTAs have several rows on their way
+    rng = np.random.default_rng(4)
+    x = values(rng, rows, width, torch.bfloat16)
+    w = dev(rng.standard_normal(width).astype(np.float32))
+    results = []
+    for place in (torch.zeros_like(x), x.clone()):
+        source = x if not results else place
+        kwargs = {}
+        if block is not None:
+            kwargs = dict(payload=torch.zeros(rows, width, dtype=torch.int8, device="cuda"), block_size=block,
+                          scales=torch.zeros(rows * (width // 32 if block else 1), device="cuda"))
+        RmsNorm.forward(0, source, w, EPS, y=place, **kwargs)
+        torch.cuda.synchronize()
+        results.append(place)
+    assert torch.equal(results[0], results[1])
+
+
 def test_without_a_residual_and_bits_for_bf16(cuda):
     rng = np.random.default_rng(4)
     x = values(rng, 6, 256, torch.bfloat16)

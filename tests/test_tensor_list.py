@@ -12,10 +12,12 @@ TENSOR = GradientTensorList._TENSOR
 
 
 def table_of(lengths, kind=0, block=0):
+    """Tensors of these lengths, one behind the other in an address space of their own."""
     table = np.zeros(len(lengths), dtype=TENSOR)
-    table["values"], table["length"], table["kind"], table["block_size"] = 4096, lengths, kind, block
+    table["length"], table["kind"], table["block_size"] = lengths, kind, block
+    table["values"] = 4096 + np.concatenate([[0], np.cumsum(lengths)[:-1]]).astype(np.uint64) * 4
     if kind == 2:
-        table["scales"] = 4096
+        table["scales"] = table["values"] + np.uint64(1 << 60)
     return table
 
 
@@ -74,9 +76,43 @@ def test_plan_refusals(lib):
     unscaled = table_of([10], kind=2, block=32)
     unscaled["scales"] = 0
     assert plan(lib, unscaled)[0] == INVALID
-    assert plan(lib, table_of([1 << 62, 1 << 62]))[0] == INVALID                # the sum of lengths would overflow
+    huge = table_of([4, 4])
+    huge["length"] = 1 << 62                                                    # the sum would overflow
+    assert plan(lib, huge)[0] == INVALID
     small = np.zeros((1, 2), dtype=np.int32)
     assert plan(lib, table_of([10_000]), small, 1)[0] == INVALID                # room for one chunk of three
+
+
+def test_plan_refuses_tensors_that_share_what_is_written(lib):
+    def status(**changed):
+        """Three fp32 tensors of 10 values at 0x1000, 0x2000, 0x3000; changed: field -> (tensor, value)."""
+        table = table_of([10, 10, 10])
+        table["values"] = [0x1000, 0x2000, 0x3000]
+        for field, (tensor, value) in changed.items():
+            table[field][tensor] = value
+        return plan(lib, table)[0]
+    assert status() == 0
+    assert status(destination=(0, 0x1000)) == 0                     # in place, said twice
+    assert status(destination=(0, 0x4000)) == 0
+    assert status(destination=(0, 0x2000 - 40)) == 0                # up to its neighbour
+    assert status(values=(1, 0x1000)) == INVALID                    # the same tensor twice
+    assert status(values=(1, 0x1000 + 36)) == INVALID               # one value shared
+    assert status(destination=(0, 0x1004)) == INVALID               # over itself, moved
+    assert status(destination=(0, 0x2000)) == INVALID               # over a neighbour
+    assert status(destination=(0, 0x2000 - 36)) == INVALID
+    twice = table_of([10, 10])
+    twice["values"], twice["destination"] = 0x1000, [0x3000, 0x4000]
+    assert plan(lib, twice)[0] == 0                                 # read twice, written apart
+    twice["destination"] = 0x3000
+    assert plan(lib, twice)[0] == INVALID
+    encoded = table_of([64, 64], kind=2, block=32)
+    encoded["values"], encoded["scales"] = 0x1000, [0x2000, 0x2008]
+    assert plan(lib, encoded)[0] == 0                               # a payload is only read
+    encoded["scales"] = [0x2000, 0x2004]
+    assert plan(lib, encoded)[0] == INVALID
+    empty = table_of([10, 0])
+    empty["values"] = 0x1000
+    assert plan(lib, empty)[0] == 0
 
 
 def test_clip_refusals_come_before_the_device(lib):

@@ -270,8 +270,11 @@ def test_refusals(cuda):
     with pytest.raises(ValueError, match="its length"):
         GradientTensorList(0, [x], destinations=[torch.zeros(9, device="cuda")])
     base = torch.zeros(20, device="cuda")
-    with pytest.raises(ValueError, match="overlaps"):
+    with pytest.raises(ValueError, match="overlap"):
         GradientTensorList(0, [base[:10]], destinations=[base[5:15]])
+    with pytest.raises(ValueError, match="overlap"):
+        GradientTensorList(0, [x, x])
+    GradientTensorList(0, [x, x], destinations=[base[:10], base[10:]])
     plan = GradientTensorList(0, [x])
     with pytest.raises(ValueError, match="device"):
         GradientNorm.clip_tensors(1, plan, 1.0, out)
