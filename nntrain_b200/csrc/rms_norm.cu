@@ -20,8 +20,11 @@
 // weight's gradient stays in registers until the end.  Rows too long for
 // registers are read again for each pass (they are in L1 / L2 then).
 //
-// Bound: HBM.  bf16 with residual, block 32: 7.1 bytes a value forward
-// (x, residual, h, payload, scales), 8 backward.
+// Bound.  Backward: HBM, 8 bytes a value of bf16 with residual; 32768 x 1536 in
+// 69 us, 59 of them at 6.8 TB/s and the rest the join of the weight gradient.
+// Forward: 7.1 bytes a value (x, residual, h, payload, scales; 2 more for a
+// decoded copy), but before that the instructions of the encode: 16384 x 1536
+// with the copy in 43 us, 75 % of the issue slots used, 82 % of HBM's rate.
 #include "bfp8_kernels.cuh"
 #include "operator_launch.cuh"
 

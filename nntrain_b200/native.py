@@ -440,29 +440,34 @@ class GradientTensorList:
         destinations = [None] * count if destinations is None else list(destinations)
         if count == 0 or not len(scales) == len(block_sizes) == len(destinations) == count:
             raise ValueError("a gradient list needs tensors, and one scale, block size and destination for each of them")
-        table = np.zeros(count, dtype=self._TENSOR)
+        rows = []
         for i, (t, s, block, to) in enumerate(zip(tensors, scales, block_sizes, destinations)):
-            if t.dtype not in _FLOATS + (torch.int8,):
+            length, encoded = t.numel(), t.dtype is torch.int8
+            if not encoded and t.dtype not in _FLOATS:
                 raise ValueError(f"tensor {i} must be float32, bfloat16 or an int8 payload, got {t.dtype}")
-            _require(t, t.dtype, f"tensor {i}", device)
-            encoded = t.dtype == torch.int8
-            if encoded:
+            kind = 2 if encoded else _kind(t)
+            if t.get_device() != device or not t.is_contiguous():
+                _require(t, t.dtype, f"tensor {i}", device)
+            if not encoded:
+                if s is not None:
+                    raise ValueError(f"tensor {i} is not a BFP8 payload: it has no scales")
+                scale_address, block, types, written = 0, 0, _BFLOAT16 if kind else _FLOAT32, length
+            else:
                 if s is None or block < 0:
                     raise ValueError(f"tensor {i} is a BFP8 payload: it needs its scales and block size")
                 _require(s, torch.float32, f"scales of tensor {i}", device)
-                if t.numel() and s.numel() != scale_count(t.numel(), block):
+                if length and s.numel() != scale_count(length, block):
                     raise ValueError(f"tensor {i}: payload / scale lengths do not match the descriptor")
-            elif s is not None:
-                raise ValueError(f"tensor {i} is not a BFP8 payload: it has no scales")
+                scale_address, types, written = s.data_ptr(), _FLOAT32, s.numel()
+            address = 0
             if to is not None:
-                _require(to, torch.float32 if encoded else to.dtype, f"destination of tensor {i}", device)
-                source = s if encoded else t
-                if not encoded and (to.dtype not in _FLOATS or _kind(to) != _kind(t)):
+                if to.dtype not in types:
                     raise ValueError(f"destination of tensor {i} must have its type")
-                if to.numel() != source.numel():
+                if to.numel() != written:
                     raise ValueError(f"destination of tensor {i} must have its length")
-            table[i] = (t.data_ptr(), _ptr(s) if encoded else 0, _ptr(to), t.numel(), 0,
-                        2 if encoded else _kind(t), block if encoded else 0)
+                address = _vector(to, f"destination of tensor {i}", device, written, types)
+            rows.append((t.data_ptr(), scale_address, address, length, 0, kind, block))
+        table = np.array(rows, dtype=self._TENSOR)
         chunks, values = ctypes.c_longlong(), ctypes.c_int()
         plan = load().nntrain_gradient_list_plan
         status = plan(table.ctypes.data, count, None, 0, ctypes.addressof(chunks), ctypes.addressof(values))
@@ -470,13 +475,15 @@ class GradientTensorList:
             raise ValueError("tensors and destinations of a gradient list must not overlap: what is written for one tensor "
                              "may not be read or written for another")
         check("gradient_list_plan", status)
-        chunk_map = np.zeros((max(chunks.value, 1), 2), dtype=np.int32)
-        check("gradient_list_plan", plan(table.ctypes.data, count, chunk_map.ctypes.data, chunks.value,
+        # table and chunk map in one buffer, one copy
+        buffer = np.zeros(table.nbytes + max(chunks.value, 1) * 8, dtype=np.uint8)
+        check("gradient_list_plan", plan(table.ctypes.data, count, buffer.ctypes.data + table.nbytes, chunks.value,
                                          ctypes.addressof(chunks), ctypes.addressof(values)))
+        buffer[:table.nbytes] = table.view(np.uint8)
         self.device, self.count, self.chunks, self.chunk_values = device, count, chunks.value, values.value
-        self.table = torch.from_numpy(table.view(np.uint8)).to(f"cuda:{device}")
-        self.chunk_map = torch.from_numpy(chunk_map).to(f"cuda:{device}")
-        self.table_address, self.map_address = self.table.data_ptr(), self.chunk_map.data_ptr()
+        self.buffer = torch.from_numpy(buffer).to(torch.device("cuda", device))
+        self.table_address = self.buffer.data_ptr()
+        self.map_address = self.table_address + table.nbytes
         self._held = (list(tensors), scales, destinations)
 
 
