@@ -74,12 +74,12 @@ struct LookupArguments {
     void* out;
     int* status;
     long long count, out_stride, first_value, block;
-    int width, block_shift;            // block_shift < 0: block is not a power of two; block 0: one scale
+    int width, block_shift;            // block_shift < 0: block is not a power of two; 63: one scale
     float scale;
 };
 
 __device__ __forceinline__ float table_scale(const LookupArguments& a, long long value) {
-    if (a.block == 0) return __ldg(a.scales);
+    // (one scale: block_shift is 63)
     const long long at = a.first_value + value;
     return __ldg(a.scales + (a.block_shift >= 0 ? at >> a.block_shift : at / a.block));
 }
@@ -139,22 +139,22 @@ embedding_lookup_kernel(LookupArguments a) {
                 }
             }
         }
+        T* row = out + column;
         #pragma unroll
         for (int t = 0; t < kTokens; ++t) {
             if (t >= here) break;
-            float v[8];
-            #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (token[t] < 0) {
-                    v[i] = 0.0f;
-                } else {
+            float v[8] = {};
+            if (token[t] >= 0) {
+                #pragma unroll
+                for (int i = 0; i < 8; ++i) {
                     if constexpr (kTable == kTableF32) v[i] = __uint_as_float(raw[t][i]);
                     else if constexpr (kTable == kTableBf16) v[i] = i & 1 ? bf16_high(raw[t][i / 2]) : bf16_low(raw[t][i / 2]);
                     else v[i] = __fmul_rn(byte_to_float(raw[t][i / 4] ^ 0x80808080u, i & 3), row_scale[t]);
                     v[i] = __fmul_rn(v[i], a.scale);
                 }
             }
-            store_values(out + t * a.out_stride + column, v);
+            store_values(row, v);
+            row += a.out_stride;
         }
     } else {
         #pragma unroll
@@ -752,7 +752,7 @@ int lookup(int device, int table_kind, const void* table, const float* scales, i
     if (count == 0) return static_cast<int>(cudaSuccess);
     const DeviceScope scope(device);
     if (scope.status() != cudaSuccess) return scope.status();
-    int shift = -1;
+    int shift = block_size == 0 ? 63 : -1;
     if (block_size > 0 && (block_size & (block_size - 1)) == 0)
         for (shift = 0; (1 << shift) < block_size;) ++shift;
     const LookupArguments a{Tokens{tokens, token_bytes, padding_token, vocab}, table, scales, out, token_status, count,
