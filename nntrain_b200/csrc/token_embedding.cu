@@ -219,53 +219,77 @@ __device__ void clear_piece(const SortArguments& a, long long piece) {
     for (int i = (ends + words * 16) / 2 + threadIdx.x; i < bytes / 2; i += kSortThreads) pieces[i] = 0;
 }
 
-// Ascending sort of `n` (a power of two, 64 at least) numbers in shared memory.
-// Strides up to 32 stay inside the 64 numbers of a warp's pairs, so the CTA
-// waits only around longer ones.
-__device__ void sort_shared(unsigned long long* data, int n) {
-    bool wide = true;
+// Ascending sort of `n` numbers, a power of two from 64 to kSmallSort, in one CTA.
+// Thread t of warp w holds the numbers 64 w + lane and 64 w + 32 + lane, so that
+// strides of 16 and less are shuffles, 32 is inside a thread, and only the longer
+// ones (15 of the 66 steps of 2048 numbers) go through shared memory, by turns
+// through two buffers, a barrier each.  (With every step in shared memory 2048
+// took 18 us, 512 8.5 us.)
+__device__ void sort_cta(unsigned long long& x, unsigned long long& y, int n, unsigned long long (*buffers)[kSmallSort]) {
+    const int lane = threadIdx.x & 31, first = (threadIdx.x >> 5) * 64 + lane, second = first + 32;
+    const bool here = first < n;                 // whole warps
+    int turn = 0;
+    const auto keep = [](unsigned long long mine, unsigned long long other, int at, int j, int k) {
+        const bool smaller = ((at & j) == 0) == ((at & k) == 0);
+        return (mine < other) == smaller ? mine : other;
+    };
     for (int k = 2; k <= n; k <<= 1) {
         for (int j = k >> 1; j > 0; j >>= 1) {
-            if (wide || j > 32) __syncthreads();
-            else __syncwarp();
-            wide = j > 32;
-            const int t = threadIdx.x;
-            if (t < n / 2) {
-                const int i = 2 * t - (t & (j - 1));
-                const unsigned long long x = data[i], y = data[i + j];
-                if ((x > y) == ((i & k) == 0)) {
-                    data[i] = y;
-                    data[i + j] = x;
+            if (j > 32) {
+                unsigned long long* data = buffers[turn];
+                turn ^= 1;
+                if (here) {
+                    data[first] = x;
+                    data[second] = y;
                 }
+                __syncthreads();
+                if (here) {
+                    x = keep(x, data[first ^ j], first, j, k);
+                    y = keep(y, data[second ^ j], second, j, k);
+                }
+            } else if (j == 32) {
+                const unsigned long long low = x < y ? x : y, high = x < y ? y : x;
+                const bool ascending = (first & k) == 0;
+                x = ascending ? low : high;
+                y = ascending ? high : low;
+            } else {
+                x = keep(x, __shfl_xor_sync(0xffffffffu, x, j), first, j, k);
+                y = keep(y, __shfl_xor_sync(0xffffffffu, y, j), second, j, k);
             }
         }
     }
-    __syncthreads();
 }
 
 // Up to kSmallSort tokens, `padded` a power of two.  Positions without a token
 // get the row `vocab`, behind all rows.
 __global__ void __launch_bounds__(kSortThreads)
 embedding_small_sort_kernel(SortArguments a, int padded) {
-    __shared__ unsigned long long pairs[kSmallSort];
-    static_assert(kSmallSort == 2 * kSortThreads, "a pair of numbers for each thread");
+    __shared__ unsigned long long buffers[2][kSmallSort];
+    static_assert(kSmallSort == 2 * kSortThreads, "two numbers for each thread");
     let_next_start();
     if (blockIdx.x > 0) {
         clear_piece(a, blockIdx.x - 1);
         return;
     }
+    const int first = (threadIdx.x >> 5) * 64 + (threadIdx.x & 31);
     bool bad = false;
-    for (int i = threadIdx.x; i < padded; i += kSortThreads) {
+    const auto load = [&](int i) {
         const long long token = i < static_cast<int>(a.count) ? a.tokens.at(i, bad) : -1;
-        pairs[i] = (static_cast<unsigned long long>(token < 0 ? a.tokens.vocab : token) << 32) | static_cast<unsigned>(i);
-    }
+        return (static_cast<unsigned long long>(token < 0 ? a.tokens.vocab : token) << 32) | static_cast<unsigned>(i);
+    };
+    unsigned long long pair[2] = {load(first), load(first + 32)};
     if (threadIdx.x < 2) a.crossing[threadIdx.x] = 0;
-    if (a.named != nullptr)
+    if (a.named != nullptr) {
         for (long long i = threadIdx.x; i * 32 < a.tokens.vocab; i += kSortThreads) a.named[i] = 0;
-    sort_shared(pairs, padded);                              // (its barriers are behind the zeros)
-    for (int i = threadIdx.x; i < static_cast<int>(a.count); i += kSortThreads) {
-        const unsigned row = static_cast<unsigned>(pairs[i] >> 32);
-        a.pairs[0][i] = make_uint2(row, static_cast<unsigned>(pairs[i]));
+        __syncthreads();
+    }
+    sort_cta(pair[0], pair[1], padded, buffers);
+    #pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int at = first + 32 * h;
+        if (at >= static_cast<int>(a.count)) continue;
+        const unsigned row = static_cast<unsigned>(pair[h] >> 32);
+        a.pairs[0][at] = make_uint2(row, static_cast<unsigned>(pair[h]));
         if (a.named != nullptr && row < a.tokens.vocab) atomicOr(a.named + (row >> 5), 1u << (row & 31u));
     }
     if (bad && a.status != nullptr) atomicExch(a.status, 1);
@@ -419,8 +443,10 @@ embedding_sort_kernel(SortArguments a) {
 
 // ---- rows and join --------------------------------------------------------------
 
-// Sorted positions of a warp.  32, so that few tokens cross; 16 where that
-// leaves the SMs less than 16 warps each.
+// Sorted positions of a warp.  32, so that few tokens cross; 16 where 32 leave
+// the 148 SMs less than 64 warps of 256 columns each (added gradients: 65536
+// tokens x 512 72 us with 16, 74 us with 32, 76 us with 8; 131072 x 768 124, 120
+// and 141 us).
 constexpr int kChunkMost = 32, kChunkLeast = 16;
 constexpr int kZeroRows = 32;                   // rows of a CTA that writes late zeros: one word of the bitmap
 // Columns of a warp: one 128-bit load of a lane, or 8 single values.
@@ -458,39 +484,47 @@ __device__ __forceinline__ float value_of(T raw) {
     else return bf16_value(raw);
 }
 
-// table[row] = scale * sum (+ what is there), rounded once.
+// What is there in a row of the table, to be added to.
 template <typename T, int kValues, bool kVector>
-__device__ __forceinline__ void store_row(const RowsArguments& a, unsigned row, int first, int lane, const float (&sum)[kValues]) {
-    T* out = static_cast<T*>(a.table) + static_cast<long long>(row) * a.width;
-    if constexpr (kVector) {
-        const int column = lane_column<kValues, true>(first, lane, 0);
-        if (column >= a.width) return;
-        out += column;
-        #pragma unroll
-        for (int q = 0; q < kValues; q += 4) {
-            float x[4] = {};
-            if (a.accumulate) {
-                if constexpr (sizeof(T) == 4) {
-                    const float4 old = load_f4(out + q);
-                    x[0] = old.x; x[1] = old.y; x[2] = old.z; x[3] = old.w;
-                } else {
-                    const uint2 old = *reinterpret_cast<const uint2*>(out + q);
-                    x[0] = bf16_low(old.x); x[1] = bf16_high(old.x); x[2] = bf16_low(old.y); x[3] = bf16_high(old.y);
-                }
-            }
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = a.accumulate ? __fmaf_rn(sum[q + i], a.scale, x[i]) : __fmul_rn(sum[q + i], a.scale);
-            if constexpr (sizeof(T) == 4) store_f4(out + q, make_float4(x[0], x[1], x[2], x[3]));
-            else *reinterpret_cast<uint2*>(out + q) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+__device__ __forceinline__ void load_old(const RowsArguments& a, unsigned row, int first, int lane, float (&old)[kValues]) {
+    const T* p = static_cast<const T*>(a.table) + static_cast<long long>(row) * a.width;
+    #pragma unroll
+    for (int i = 0; i < kValues; i += kVector ? 4 : 1) {
+        const int column = lane_column<kValues, kVector>(first, lane, i);
+        if constexpr (!kVector) {
+            old[i] = column < a.width ? value_of(p[column]) : 0.0f;
+        } else if constexpr (sizeof(T) == 4) {
+            const float4 x = column < a.width ? load_f4(p + column) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            old[i] = x.x; old[i + 1] = x.y; old[i + 2] = x.z; old[i + 3] = x.w;
+        } else {
+            const uint2 x = column < a.width ? *reinterpret_cast<const uint2*>(p + column) : make_uint2(0, 0);
+            old[i] = bf16_low(x.x); old[i + 1] = bf16_high(x.x); old[i + 2] = bf16_low(x.y); old[i + 3] = bf16_high(x.y);
         }
-    } else {
+    }
+}
+
+// table[row] = scale * sum (+ old), rounded once.
+template <typename T, int kValues, bool kVector, bool kAdd>
+__device__ __forceinline__ void store_row(const RowsArguments& a, unsigned row, int first, int lane, const float (&sum)[kValues],
+                                          const float (&old)[kAdd ? kValues : 1]) {
+    T* out = static_cast<T*>(a.table) + static_cast<long long>(row) * a.width;
+    #pragma unroll
+    for (int i = 0; i < kValues; i += kVector ? 4 : 1) {
+        const int column = lane_column<kValues, kVector>(first, lane, i);
+        if (column >= a.width) continue;
+        float x[kVector ? 4 : 1];
         #pragma unroll
-        for (int i = 0; i < kValues; ++i) {
-            const int column = lane_column<kValues, false>(first, lane, i);
-            if (column >= a.width) continue;
-            const float x = a.accumulate ? __fmaf_rn(sum[i], a.scale, value_of(out[column])) : __fmul_rn(sum[i], a.scale);
-            if constexpr (sizeof(T) == 4) out[column] = x;
-            else out[column] = bf16_bits(x);
+        for (int q = 0; q < (kVector ? 4 : 1); ++q) {
+            if constexpr (kAdd) x[q] = __fmaf_rn(sum[i + q], a.scale, old[i + q]);
+            else x[q] = __fmul_rn(sum[i + q], a.scale);
+        }
+        if constexpr (!kVector) {
+            if constexpr (sizeof(T) == 4) out[column] = x[0];
+            else out[column] = bf16_bits(x[0]);
+        } else if constexpr (sizeof(T) == 4) {
+            store_f4(out + column, make_float4(x[0], x[1], x[2], x[3]));
+        } else {
+            *reinterpret_cast<uint2*>(out + column) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
         }
     }
 }
@@ -530,7 +564,7 @@ __device__ void zero_rows(const RowsArguments& a, unsigned group) {
 // not a warp.
 constexpr unsigned kLongChunks = 16;
 
-template <typename G, typename T, bool kVector>
+template <typename G, typename T, bool kVector, bool kAdd>
 __global__ void __launch_bounds__(kThreads)
 embedding_rows_kernel(RowsArguments a) {
     constexpr int kValues = lane_values<G, kVector>();
@@ -551,17 +585,24 @@ embedding_rows_kernel(RowsArguments a) {
     const unsigned key_before = chunk > 0 ? a.pairs[base - 1].x : a.vocab;
     const unsigned key_behind = base + size < a.count ? a.pairs[base + size].x : a.vocab;
     const int n = __popc(__ballot_sync(0xffffffffu, key != a.vocab));    // rows come first
-    constexpr int kBatch = kVector ? 8 : 4;          // rows whose loads are in flight together
+    // Rows whose loads are in flight together; when adding, with the rows of the table that they complete (one after
+    // the other these were most of a warp's time: 15 us for 16 tokens, XX us so).
+    constexpr int kBatch = kVector && !kAdd ? 8 : 4;
     const G* gradient = static_cast<const G*>(a.gradient);
     float sum[kValues] = {};
-    bool begun_here = __shfl_sync(0xffffffffu, key, 0) != key_before;
+    const unsigned following = __shfl_down_sync(0xffffffffu, key, 1);
+    const unsigned next_key = lane + 1 < static_cast<int>(size) ? following : key_behind;
     for (int j = 0; j < n; j += kBatch) {
         uint4 raw[kBatch];
+        float old[kBatch][kAdd ? kValues : 1];
         G single[kBatch][kValues];
         #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             const unsigned at = __shfl_sync(0xffffffffu, position, (j + b) & 31);
+            const unsigned here = __shfl_sync(0xffffffffu, key, (j + b) & 31), next = __shfl_sync(0xffffffffu, next_key, (j + b) & 31);
             if (j + b >= n) continue;
+            if constexpr (kAdd)
+                if (here != next && here != key_before) load_old<T, kValues, kVector>(a, here, first, lane, old[b]);
             const G* row = gradient + static_cast<long long>(at) * a.gradient_stride;
             if constexpr (kVector) {
                 const int column = lane_column<kValues, true>(first, lane, 0);
@@ -577,8 +618,7 @@ embedding_rows_kernel(RowsArguments a) {
         #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             if (j + b >= n) continue;
-            const unsigned here = __shfl_sync(0xffffffffu, key, j + b);
-            const unsigned next = j + b + 1 < static_cast<int>(size) ? __shfl_sync(0xffffffffu, key, (j + b + 1) & 31) : key_behind;
+            const unsigned here = __shfl_sync(0xffffffffu, key, j + b), next = __shfl_sync(0xffffffffu, next_key, j + b);
             if constexpr (kVector) {
                 const unsigned w[4] = {raw[b].x, raw[b].y, raw[b].z, raw[b].w};
                 #pragma unroll
@@ -595,19 +635,19 @@ embedding_rows_kernel(RowsArguments a) {
                 for (int i = 0; i < kValues; ++i) sum[i] = __fadd_rn(sum[i], value_of(single[b][i]));
             }
             if (next == here && j + b + 1 < static_cast<int>(size)) continue;      // the token goes on in this chunk
+            const bool begun_before = here == key_before;
             if (next == here) {
                 store_partial<kValues, kVector>(a.tails, chunk, a.width, first, lane, sum);
-                if (begun_here && first == 0 && lane == 0) {
+                if (!begun_before && first == 0 && lane == 0) {
                     const unsigned long long far = static_cast<unsigned long long>(chunk + kLongChunks) * size;
                     const bool is_long = far < a.count && a.pairs[far].x == here;
                     (is_long ? a.crossing_long : a.crossing_short)[atomicAdd(a.crossing + is_long, 1u)] = chunk;
                 }
-            } else if (!begun_here) {
+            } else if (begun_before) {
                 store_partial<kValues, kVector>(a.heads, chunk, a.width, first, lane, sum);
             } else {
-                store_row<T, kValues, kVector>(a, here, first, lane, sum);
+                store_row<T, kValues, kVector, kAdd>(a, here, first, lane, sum, old[b]);
             }
-            begun_here = true;
             #pragma unroll
             for (int i = 0; i < kValues; ++i) sum[i] = 0.0f;
         }
@@ -668,7 +708,7 @@ __device__ __forceinline__ void add_partials(const RowsArguments& a, unsigned be
 // The first CTAs take the long crossing tokens (and a slice of their columns):
 // each of 8 warps adds an eighth of the partials in order, the eighths are
 // added in order.  In the others a warp takes a short one.
-template <typename T, int kValues, bool kVector>
+template <typename T, int kValues, bool kVector, bool kAdd>
 __global__ void __launch_bounds__(kThreads)
 embedding_join_kernel(RowsArguments a) {
     __shared__ float sums[kWarpsPerCta][kValues * 32];
@@ -687,10 +727,12 @@ embedding_join_kernel(RowsArguments a) {
         const int first = static_cast<int>(task % a.slices) * (kValues * 32);
         const unsigned key = a.pairs[begin * a.chunk + a.chunk - 1].x;
         const unsigned end = last_chunk_of(a, key, begin, lane), parts = end - begin + 1;
-        float sum[kValues] = {};
+        float sum[kValues] = {}, old[kAdd ? kValues : 1];
+        if constexpr (kAdd)
+            if (!is_long || warp == 0) load_old<T, kValues, kVector>(a, key, first, lane, old);
         if (!is_long) {
             add_partials<kValues, kVector>(a, begin, end, 0, parts, first, lane, sum);
-            store_row<T, kValues, kVector>(a, key, first, lane, sum);
+            store_row<T, kValues, kVector, kAdd>(a, key, first, lane, sum, old);
             continue;
         }
         const unsigned share = (parts + kWarpsPerCta - 1) / kWarpsPerCta;
@@ -704,7 +746,7 @@ embedding_join_kernel(RowsArguments a) {
                 #pragma unroll
                 for (int i = 0; i < kValues; ++i) sum[i] = __fadd_rn(sum[i], sums[w][i * 32 + lane]);
             }
-            store_row<T, kValues, kVector>(a, key, first, lane, sum);
+            store_row<T, kValues, kVector, kAdd>(a, key, first, lane, sum, old);
         }
         __syncthreads();
     }
@@ -784,9 +826,8 @@ GradientScratch gradient_scratch(long long count, long long vocab, int width) {
         s.bytes += (bytes + 255) / 256 * 256;
         return at;
     };
-    // (256 columns a warp; with 148 SMs this is 16 warps each)
     const long long warps = (count + kChunkMost - 1) / kChunkMost * ((width + 255) / 256);
-    s.chunk = warps < 148 * 16 ? kChunkLeast : kChunkMost;
+    s.chunk = warps < 148 * 64 ? kChunkLeast : kChunkMost;
     s.chunks = (count + s.chunk - 1) / s.chunk;
     for (int i = 0; i < 2; ++i) s.pairs[i] = take(count * 8);
     s.named = take((vocab + 31) / 32 * 4);
@@ -867,7 +908,7 @@ cudaError_t launch_sort(SortArguments a, cudaStream_t stream) {
     return launch_cluster<kClusterSmall>(embedding_sort_kernel<kClusterSmall, false>, kClusterSmall, a, stream);
 }
 
-template <typename G, typename T, bool kVector>
+template <typename G, typename T, bool kVector, bool kAdd>
 cudaError_t run_rows(RowsArguments a, cudaStream_t stream) {
     constexpr int kValues = lane_values<G, kVector>();
     const long long slices = (a.width + kValues * 32 - 1) / (kValues * 32);
@@ -876,18 +917,19 @@ cudaError_t run_rows(RowsArguments a, cudaStream_t stream) {
     a.row_ctas = static_cast<int>((a.chunks * slices + kWarpsPerCta - 1) / kWarpsPerCta);
     const bool join = a.chunks > 1;
     a.join_groups = join ? a.late_groups - a.late_groups / 3 : a.late_groups;
-    const cudaError_t e = launch_dependent(embedding_rows_kernel<G, T, kVector>, a.row_ctas + static_cast<int>(a.join_groups),
+    const cudaError_t e = launch_dependent(embedding_rows_kernel<G, T, kVector, kAdd>, a.row_ctas + static_cast<int>(a.join_groups),
                                            kThreads, 0, stream, a);
     if (e != cudaSuccess || !join) return e;
     a.long_ctas = a.chunks > kLongChunks ? grid_for(a.chunks / kLongChunks * slices, 2) : 0;
     a.join_ctas = a.long_ctas + grid_for(((a.chunks - 1) * slices + kWarpsPerCta - 1) / kWarpsPerCta, 4);
-    return launch_dependent(embedding_join_kernel<T, kValues, kVector>, a.join_ctas + static_cast<int>(a.late_groups - a.join_groups),
+    return launch_dependent(embedding_join_kernel<T, kValues, kVector, kAdd>, a.join_ctas + static_cast<int>(a.late_groups - a.join_groups),
                             kThreads, 0, stream, a);
 }
 
 template <typename G, typename T>
 cudaError_t run_rows(const RowsArguments& a, bool vector_ok, cudaStream_t stream) {
-    return vector_ok ? run_rows<G, T, true>(a, stream) : run_rows<G, T, false>(a, stream);
+    if (a.accumulate) return vector_ok ? run_rows<G, T, true, true>(a, stream) : run_rows<G, T, false, true>(a, stream);
+    return vector_ok ? run_rows<G, T, true, false>(a, stream) : run_rows<G, T, false, false>(a, stream);
 }
 
 int gradient(int device, int gradient_kind, const void* out_gradient, long long gradient_stride, const void* tokens,

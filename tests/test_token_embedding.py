@@ -55,7 +55,7 @@ def test_scratch_size(lib):
     # two arrays of a pair per token, a bit per row, two counters, lists of the tokens that cross chunks of 16 or 32,
     # two rows of fp32 a chunk
     for count, vocab, width, chunk in ((0, 1, 1, 16), (1, 10, 64, 16), (32, 10, 64, 16), (33, 10, 64, 16),
-                                       (8192, 151936, 1536, 16), (65536, 32000, 512, 32)):
+                                       (8192, 151936, 1536, 16), (65536, 32000, 512, 16), (131072, 50000, 768, 32)):
         chunks = -(-count // chunk)
         parts = [count * 8] * 2 + [-(-vocab // 32) * 4, 8, chunks * 4, (chunks // 16 + 1) * 4] + [chunks * width * 4] * 2
         assert size(count, vocab, width) == sum(-(-p // 256) * 256 for p in parts)
