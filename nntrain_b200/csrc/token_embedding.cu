@@ -181,7 +181,7 @@ embedding_lookup_kernel(LookupArguments a) {
 
 // ---- sort ---------------------------------------------------------------------
 
-constexpr int kSmallSort = 2048;                // tokens that one CTA sorts
+constexpr int kSmallBits = 11, kSmallSort = 1 << kSmallBits;   // tokens that one CTA sorts
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 // CTAs of the sorting cluster: 8 is the portable size.  16, where the device has
 // them, for more tokens than 8 CTAs hold in one load of their warps and nothing
@@ -219,77 +219,81 @@ __device__ void clear_piece(const SortArguments& a, long long piece) {
     for (int i = (ends + words * 16) / 2 + threadIdx.x; i < bytes / 2; i += kSortThreads) pieces[i] = 0;
 }
 
-// Ascending sort of `n` numbers, a power of two from 64 to kSmallSort, in one CTA.
-// Thread t of warp w holds the numbers 64 w + lane and 64 w + 32 + lane, so that
-// strides of 16 and less are shuffles, 32 is inside a thread, and only the longer
-// ones (15 of the 66 steps of 2048 numbers) go through shared memory, by turns
-// through two buffers, a barrier each.  (With every step in shared memory 2048
-// took 18 us, 512 8.5 us.)
-__device__ void sort_cta(unsigned long long& x, unsigned long long& y, int n, unsigned long long (*buffers)[kSmallSort]) {
+// Ascending sort of `n` numbers, a power of two from 64 to kSmallSort, by the
+// warps of a CTA that hold them.  Thread t of warp w has the numbers 64 w + lane
+// and 64 w + 32 + lane, so that strides of 16 and less are shuffles, 32 is inside
+// a thread, and only the longer ones (15 of the 66 steps of 2048 numbers) go
+// through shared memory, by turns through two buffers, a barrier each.  Bound by
+// the instructions of the shuffles: 10 us for 2048, 18 us with every step in
+// shared memory.
+template <typename K>
+__device__ void sort_cta(K& x, K& y, int n, K (*buffers)[kSmallSort]) {
     const int lane = threadIdx.x & 31, first = (threadIdx.x >> 5) * 64 + lane, second = first + 32;
-    const bool here = first < n;                 // whole warps
-    int turn = 0;
-    const auto keep = [](unsigned long long mine, unsigned long long other, int at, int j, int k) {
-        const bool smaller = ((at & j) == 0) == ((at & k) == 0);
-        return (mine < other) == smaller ? mine : other;
+    const auto keep = [](K mine, K other, bool smaller) {
+        const K low = mine < other ? mine : other, high = mine < other ? other : mine;
+        return smaller ? low : high;
     };
+    int turn = 0;
     for (int k = 2; k <= n; k <<= 1) {
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            if (j > 32) {
-                unsigned long long* data = buffers[turn];
-                turn ^= 1;
-                if (here) {
-                    data[first] = x;
-                    data[second] = y;
-                }
-                __syncthreads();
-                if (here) {
-                    x = keep(x, data[first ^ j], first, j, k);
-                    y = keep(y, data[second ^ j], second, j, k);
-                }
-            } else if (j == 32) {
-                const unsigned long long low = x < y ? x : y, high = x < y ? y : x;
-                const bool ascending = (first & k) == 0;
-                x = ascending ? low : high;
-                y = ascending ? high : low;
-            } else {
-                x = keep(x, __shfl_xor_sync(0xffffffffu, x, j), first, j, k);
-                y = keep(y, __shfl_xor_sync(0xffffffffu, y, j), second, j, k);
-            }
+        const bool x_up = (first & k) == 0, y_up = (second & k) == 0;
+        for (int j = k >> 1; j > 32; j >>= 1) {
+            K* data = buffers[turn];
+            turn ^= 1;
+            data[first] = x;
+            data[second] = y;
+            __syncthreads();
+            x = keep(x, data[first ^ j], ((first & j) == 0) == x_up);
+            y = keep(y, data[second ^ j], ((second & j) == 0) == y_up);
+        }
+        if (k >= 64) {
+            const K low = x < y ? x : y, high = x < y ? y : x;
+            x = x_up ? low : high;
+            y = x_up ? high : low;
+        }
+        #pragma unroll
+        for (int j = 16; j > 0; j >>= 1) {
+            if (j >= k) continue;
+            const bool lower = (lane & j) == 0;
+            x = keep(x, __shfl_xor_sync(0xffffffffu, x, j), lower == x_up);
+            y = keep(y, __shfl_xor_sync(0xffffffffu, y, j), lower == y_up);
         }
     }
 }
 
 // Up to kSmallSort tokens, `padded` a power of two.  Positions without a token
-// get the row `vocab`, behind all rows.
+// get the row `vocab`, behind all rows.  K holds a row above kPositionBits of
+// its position: 32 bits where they suffice.
+template <typename K>
 __global__ void __launch_bounds__(kSortThreads)
 embedding_small_sort_kernel(SortArguments a, int padded) {
-    __shared__ unsigned long long buffers[2][kSmallSort];
-    static_assert(kSmallSort == 2 * kSortThreads, "two numbers for each thread");
+    constexpr int kPositionBits = sizeof(K) == 4 ? kSmallBits : 32;
+    __shared__ K buffers[2][kSmallSort];
+    static_assert(kSmallSort == 2 * kSortThreads && kSmallSort == 1 << kSmallBits, "two numbers for each thread");
     let_next_start();
     if (blockIdx.x > 0) {
         clear_piece(a, blockIdx.x - 1);
         return;
     }
-    const int first = (threadIdx.x >> 5) * 64 + (threadIdx.x & 31);
-    bool bad = false;
-    const auto load = [&](int i) {
-        const long long token = i < static_cast<int>(a.count) ? a.tokens.at(i, bad) : -1;
-        return (static_cast<unsigned long long>(token < 0 ? a.tokens.vocab : token) << 32) | static_cast<unsigned>(i);
-    };
-    unsigned long long pair[2] = {load(first), load(first + 32)};
     if (threadIdx.x < 2) a.crossing[threadIdx.x] = 0;
     if (a.named != nullptr) {
         for (long long i = threadIdx.x; i * 32 < a.tokens.vocab; i += kSortThreads) a.named[i] = 0;
         __syncthreads();
     }
-    sort_cta(pair[0], pair[1], padded, buffers);
+    const int first = (threadIdx.x >> 5) * 64 + (threadIdx.x & 31);
+    if (first >= padded) return;                 // whole warps; barriers wait for those that are left
+    bool bad = false;
+    const auto load = [&](int i) {
+        const long long token = i < static_cast<int>(a.count) ? a.tokens.at(i, bad) : -1;
+        return (static_cast<K>(token < 0 ? a.tokens.vocab : token) << kPositionBits) | static_cast<K>(i);
+    };
+    K pair[2] = {load(first), load(first + 32)};
+    sort_cta<K>(pair[0], pair[1], padded, buffers);
     #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int at = first + 32 * h;
         if (at >= static_cast<int>(a.count)) continue;
-        const unsigned row = static_cast<unsigned>(pair[h] >> 32);
-        a.pairs[0][at] = make_uint2(row, static_cast<unsigned>(pair[h]));
+        const unsigned row = static_cast<unsigned>(pair[h] >> kPositionBits);
+        a.pairs[0][at] = make_uint2(row, static_cast<unsigned>(pair[h] & ((static_cast<K>(1) << kPositionBits) - 1)));
         if (a.named != nullptr && row < a.tokens.vocab) atomicOr(a.named + (row >> 5), 1u << (row & 31u));
     }
     if (bad && a.status != nullptr) atomicExch(a.status, 1);
@@ -586,7 +590,7 @@ embedding_rows_kernel(RowsArguments a) {
     const unsigned key_behind = base + size < a.count ? a.pairs[base + size].x : a.vocab;
     const int n = __popc(__ballot_sync(0xffffffffu, key != a.vocab));    // rows come first
     // Rows whose loads are in flight together; when adding, with the rows of the table that they complete (one after
-    // the other these were most of a warp's time: 15 us for 16 tokens, XX us so).
+    // the other these were most of a warp's time: 15 us for 300 tokens, 9 us so).
     constexpr int kBatch = kVector && !kAdd ? 8 : 4;
     const G* gradient = static_cast<const G*>(a.gradient);
     float sum[kValues] = {};
@@ -894,7 +898,11 @@ cudaError_t launch_sort(SortArguments a, cudaStream_t stream) {
     if (a.count <= kSmallSort) {
         int padded = 64;
         while (padded < static_cast<int>(a.count)) padded <<= 1;
-        embedding_small_sort_kernel<<<static_cast<unsigned>(1 + pieces), kSortThreads, 0, stream>>>(a, padded);
+        const unsigned ctas = static_cast<unsigned>(1 + pieces);
+        if (a.tokens.vocab < 1ll << (32 - kSmallBits))
+            embedding_small_sort_kernel<unsigned><<<ctas, kSortThreads, 0, stream>>>(a, padded);
+        else
+            embedding_small_sort_kernel<unsigned long long><<<ctas, kSortThreads, 0, stream>>>(a, padded);
         return cudaPeekAtLastError();
     }
     a.passes = 1;                                // over the bits of the largest key, `vocab`

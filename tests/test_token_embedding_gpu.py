@@ -200,6 +200,23 @@ def test_every_number_of_passes_sorts(cuda, vocab):
         check_gradient(tokens, dev(dout), got, 1.0, vocab)
 
 
+@pytest.mark.parametrize("vocab", (3, 1000, (1 << 21) - 1, 1 << 21, (1 << 21) + 7))
+@pytest.mark.parametrize("count", (1, 2, 63, 64, 65, 500, 1024, 1025, 2047, 2048, 2049))
+def test_small_sorts(cuda, vocab, count):
+    """One CTA's sort at its borders, with 32- and 64-bit keys."""
+    rng = np.random.default_rng(count)
+    tokens = some_tokens(rng, count, vocab, 0.1, "even" if vocab > 1000 else "text")
+    dout = dev(rng.standard_normal((count, 4)).astype(np.float32))
+    before = torch.ones(vocab, 4, device="cuda")
+    got = before.clone()
+    TokenEmbedding.gradient(0, dev(tokens), dout, got, accumulate=True)
+    whole = torch.full((vocab, 4), 9.0, device="cuda")
+    TokenEmbedding.gradient(0, dev(tokens), dout, whole)
+    torch.cuda.synchronize()
+    check_gradient(tokens, dout, got, 1.0, vocab, before)
+    check_gradient(tokens, dout, whole, 1.0, vocab)
+
+
 @pytest.mark.parametrize("vocab,width", ((70000, 4), (300_000, 4), (1 << 28, 1)))
 def test_one_bucket_takes_all(cuda, vocab, width):
     """Rows that agree in their low 9 bits: one, two and three passes over the others."""
