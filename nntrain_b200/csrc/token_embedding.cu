@@ -435,7 +435,7 @@ embedding_sort_kernel(SortArguments a) {
             const unsigned digit = (pair.x >> shift) & (kDigits - 1), same = same_digit(here, digit);
             const unsigned before = same & below_lane;
             const unsigned place = here ? starts[digit] + mine[digit] + __popc(before) : a.count;
-            if (place < a.count) out[place] = pair;          // (it is, unless the tokens change while they are sorted)
+            if (place < a.count) out[place] = pair;          // (it is, unless the tokens are written meanwhile)
             __syncwarp();
             if (here && before == 0) mine[digit] += __popc(same);
             __syncwarp();
@@ -585,10 +585,12 @@ embedding_rows_kernel(RowsArguments a) {
     const int first = static_cast<int>(task - chunk * a.slices) * (kValues * 32);
     const uint2 none = make_uint2(a.vocab, 0);
     const uint2 pair = lane < static_cast<int>(size) && base + lane < a.count ? a.pairs[base + lane] : none;
-    const unsigned key = pair.x, position = pair.y;
+    // (the sort leaves rows and positions; tokens that are written while they are sorted must not lead out of the table)
+    const unsigned key = pair.x < a.vocab ? pair.x : a.vocab, position = pair.y < a.count ? pair.y : 0;
     const unsigned key_before = chunk > 0 ? a.pairs[base - 1].x : a.vocab;
     const unsigned key_behind = base + size < a.count ? a.pairs[base + size].x : a.vocab;
-    const int n = __popc(__ballot_sync(0xffffffffu, key != a.vocab));    // rows come first
+    const unsigned named = __ballot_sync(0xffffffffu, key != a.vocab);       // rows come first
+    const int n = named == 0xffffffffu ? 32 : __ffs(static_cast<int>(~named)) - 1;
     // Rows whose loads are in flight together; when adding, with the rows of the table that they complete (one after
     // the other these were most of a warp's time: 15 us for 300 tokens, 9 us so).
     constexpr int kBatch = kVector && !kAdd ? 8 : 4;

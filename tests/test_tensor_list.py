@@ -134,6 +134,20 @@ def test_clip_refusals_come_before_the_device(lib):
         assert call(max_norm=max_norm) == INVALID
 
 
+def test_refused_calls_land_in_the_error_ring(lib):
+    from nntrain_b200.library import last_error
+    chunks, values = ctypes.c_longlong(), ctypes.c_int()
+    for operation, call in (
+            (219, lambda: lib.nntrain_gradient_list_plan(None, 1, None, 0, ctypes.addressof(chunks), ctypes.addressof(values))),
+            (219, lambda: lib.nntrain_gradient_list_clip(0, None, 1, None, 0, 4096, None, 1.0, 1, None, None, None, None)),
+            (220, lambda: lib.nntrain_rms_norm_backward_workspace(-1, 1, None)),
+            (221, lambda: lib.nntrain_embedding_gradient_workspace(-1, 1, 1, None))):
+        before = last_error().sequence
+        assert call() == INVALID
+        info = last_error()
+        assert info.sequence == before + 1 and info.operation == operation and info.status == INVALID
+
+
 def test_a_list_refuses_tensors_that_are_not_on_a_device():
     import torch
     with pytest.raises(ValueError, match="CUDA"):

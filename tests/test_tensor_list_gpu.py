@@ -205,6 +205,18 @@ def test_same_list_same_bits(cuda):
         assert r[:2] == results[0][:2] and torch.equal(r[2], results[0][2])
 
 
+@pytest.mark.parametrize("lengths", ((70_001, 5, 300), (9_000_000, 4096)))
+def test_the_norm_alone_and_with_the_clip_has_the_same_bits(cuda, lengths):
+    """Short lists are summed by the clip's blocks, long ones by a block of their own: one order."""
+    rng = np.random.default_rng(10)
+    plan, results = as_list([Leaf(rng, n, "f32") for n in lengths]), []
+    for apply in (False, True):
+        out, norms = torch.zeros(2, device="cuda"), torch.zeros(len(lengths), device="cuda")
+        GradientNorm.clip_tensors(0, plan, 0.1, out, norms, apply=apply)
+        results.append((host(out).tobytes(), host(norms).tobytes()))
+    assert results[0] == results[1]
+
+
 def test_a_list_longer_than_the_smallest_chunks(cuda):
     """300 M values: the longest chunks, over 12 000 of them, several for a finishing lane."""
     n = 300_000_001
