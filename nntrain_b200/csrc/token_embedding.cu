@@ -184,13 +184,18 @@ embedding_lookup_kernel(LookupArguments a) {
 constexpr int kSmallBits = 11, kSmallSort = 1 << kSmallBits;   // tokens that one CTA sorts
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 // CTAs of the sorting cluster: 8 is the portable size.  16, where the device has
-// them, for more tokens than 8 CTAs hold in one load of their warps and nothing
-// beside the sort to hide it (65536 tokens: 35 us with 8, 24 us with 16).
+// them, for more tokens than 8 CTAs hold in their registers and no long clearing
+// beside the sort to hide it (65536 tokens added to a table: 76 us with 8, 65 us with 16).
 constexpr int kClusterSmall = 8, kClusterLarge = 16;
-constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
-constexpr int kSteps = 4;                       // groups of 32 tokens that a warp loads ahead
-constexpr int kSortShared = (kSortWarps + 2) * kDigits * 4;
-constexpr long long kClearBytes = 128 << 10;    // of a CTA beside the sort: 8 stores of a thread; 805 MB at 7.3 TB/s
+constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;   // of a pass at most
+constexpr int kLeastBits = 5;                   // a warp of digits
+template <int kCluster>
+constexpr int sort_shared() { return (kSortWarps + 2 + kCluster) * kDigits * 4; }
+// Zeros of a CTA beside the sort; and from how many bytes on, these and some for
+// each token, they take longer than the sort (8192 tokens, 197 MB: 59 us with two
+// CTAs of an SM, 61 us with one; 30000 tokens, 307 MB: 106 and 98 us; 65536
+// tokens, 98 MB: 98 and 83 us).
+constexpr long long kClearPiece = 128 << 10, kClearLong = 128ll << 20, kClearToken = 6 << 10;
 
 struct SortArguments {
     Tokens tokens;
@@ -199,16 +204,16 @@ struct SortArguments {
     unsigned* named;                   // a bit for each row, set where a token names it; null when not asked for
     int* status;
     char* clear;                       // bytes that the CTAs behind the sort's clear
-    long long clear_bytes;
+    long long clear_bytes, clear_piece;          // all of them, and those of a CTA
     unsigned count;
-    int passes;
+    int passes, bits;                  // and the bits of a pass's digit
 };
 
 // Zeros to the piece number `piece` of a.clear.  (A table is whole values, so
 // its unaligned ends are whole 2-byte pieces.)
 __device__ void clear_piece(const SortArguments& a, long long piece) {
-    char* begin = a.clear + piece * kClearBytes;
-    const long long left = a.clear_bytes - piece * kClearBytes, bytes = left < kClearBytes ? left : kClearBytes;
+    char* begin = a.clear + piece * a.clear_piece;
+    const long long left = a.clear_bytes - piece * a.clear_piece, bytes = left < a.clear_piece ? left : a.clear_piece;
     const int head = static_cast<int>((16u - (reinterpret_cast<std::uintptr_t>(begin) & 15u)) & 15u);
     const int ends = head < bytes ? head : static_cast<int>(bytes);
     const int words = static_cast<int>((bytes - ends) / 16);
@@ -300,13 +305,14 @@ embedding_small_sort_kernel(SortArguments a, int padded) {
 }
 
 // The first kSteps groups of 32 pairs of a warp's stretch.
+template <int kSteps>
 struct Head {
     uint2 pairs[kSteps];
 };
 
-template <typename Load>
-__device__ __forceinline__ Head load_head(unsigned from, unsigned to, Load load) {
-    Head head;
+template <int kSteps, typename Load>
+__device__ __forceinline__ Head<kSteps> load_head(unsigned from, unsigned to, Load load) {
+    Head<kSteps> head;
     #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
         const unsigned at = from + s * 32 + (threadIdx.x & 31);
@@ -317,11 +323,11 @@ __device__ __forceinline__ Head load_head(unsigned from, unsigned to, Load load)
 
 // Walks [from, to) 32 at a time, in order: visit(here, pair).  kSteps groups are
 // loaded before the first of them is visited; the first ones are there already.
-template <typename Load, typename Visit>
-__device__ __forceinline__ void walk(unsigned from, unsigned to, Head head, Load load, Visit visit) {
+template <int kSteps, typename Load, typename Visit>
+__device__ __forceinline__ void walk(unsigned from, unsigned to, Head<kSteps> head, Load load, Visit visit) {
     const int lane = threadIdx.x & 31;
     for (unsigned base = from; base < to; base += 32 * kSteps) {
-        if (base != from) head = load_head(base, to, load);
+        if (base != from) head = load_head<kSteps>(base, to, load);
         #pragma unroll
         for (int s = 0; s < kSteps; ++s)
             if (base + s * 32 < to) visit(base + s * 32 + lane < to, head.pairs[s]);
@@ -329,10 +335,11 @@ __device__ __forceinline__ void walk(unsigned from, unsigned to, Head head, Load
 }
 
 // Lanes that are here and have the lane's digit: a vote per bit.
-__device__ __forceinline__ unsigned same_digit(bool here, unsigned digit) {
+__device__ __forceinline__ unsigned same_digit(bool here, unsigned digit, int bits) {
     unsigned same = __ballot_sync(0xffffffffu, here);
     #pragma unroll
     for (int b = 0; b < kDigitBits; ++b) {
+        if (b >= bits) break;
         const bool set = (digit >> b) & 1u;
         const unsigned votes = __ballot_sync(0xffffffffu, set);
         same &= set ? votes : ~votes;
@@ -342,23 +349,29 @@ __device__ __forceinline__ unsigned same_digit(bool here, unsigned digit) {
 
 // Stable: warps own consecutive stretches of the input, a warp walks its
 // stretch 32 at a time, and equal digits keep the order of their lanes.  A pair
-// is stored in one piece: the scattered stores of 8 SMs, a 32-byte sector each,
-// are what a pass over many tokens waits for (65536 tokens: 47 us with rows and
-// positions apart, 35 us so).
+// is stored in one piece: the scattered stores of a few SMs, a 32-byte sector
+// each, are most of a pass over many tokens (65536 tokens, 8 CTAs: 47 us with
+// rows and positions apart, 35 us so).  A stretch that fits a warp's registers is
+// ranked once, when its digits are counted, and only placed afterwards.  Every CTA
+// writes its counts into the others' shared memory in front of the barrier that
+// it needs anyway, and sums them from its own.
 //
-// kClear: CTAs behind the first cluster clear; two fit an SM then.
-template <int kCluster, bool kClear>
-__global__ void __launch_bounds__(kSortThreads, kClear ? 2 : 1)
+// CTAs behind the first cluster clear.  kResident: 2 CTAs of an SM write zeros at
+// 7.3 TB/s, one at 6.3 TB/s, but their 32 registers hold no ranks, and the sort
+// takes longer; for the tables whose zeros do.
+template <int kCluster, int kSteps, int kResident>
+__global__ void __launch_bounds__(kSortThreads, kResident)
 embedding_sort_kernel(SortArguments a) {
-    extern __shared__ unsigned shared[];
+    extern __shared__ __align__(16) unsigned shared[];
     unsigned* counts = shared;                               // [warps][digits]
-    unsigned* totals = shared + kSortWarps * kDigits;        // [digits], read by the whole cluster
+    unsigned* totals = shared + kSortWarps * kDigits;        // [digits]
     unsigned* starts = totals + kDigits;                     // [digits]
+    unsigned* shares = starts + kDigits;                     // [CTAs][digits]: the totals of each
     __shared__ unsigned sums[32];
     let_next_start();
-    if (kClear && blockIdx.x >= kCluster) {                  // whole clusters of them: no barrier is shared
+    if (blockIdx.x >= kCluster) {                            // whole clusters of them: no barrier is shared
         const long long piece = blockIdx.x - kCluster;
-        if (piece * kClearBytes < a.clear_bytes) clear_piece(a, piece);
+        if (piece * a.clear_piece < a.clear_bytes) clear_piece(a, piece);
         return;
     }
     cg::cluster_group cluster = cg::this_cluster();
@@ -367,18 +380,21 @@ embedding_sort_kernel(SortArguments a) {
     const unsigned below_lane = (1u << lane) - 1u;
     constexpr unsigned kWorkers = kCluster * kSortWarps;
     const unsigned stretch = ((a.count + kWorkers - 1) / kWorkers + 31u) & ~31u;
+    const bool held = kResident == 1 && stretch <= 32 * kSteps;
     const unsigned long long begin = static_cast<unsigned long long>(rank * kSortWarps + warp) * stretch;
     const unsigned first = begin < a.count ? static_cast<unsigned>(begin) : a.count;
     const unsigned last = begin + stretch < a.count ? static_cast<unsigned>(begin + stretch) : a.count;
+    const int digits = 1 << a.bits;
     unsigned* mine = counts + warp * kDigits;
     if (rank == 0 && threadIdx.x < 2) a.crossing[threadIdx.x] = 0;
-    if (kClear && a.named != nullptr) {
+    if (a.named != nullptr) {
         for (long long i = rank * kSortThreads + threadIdx.x; i * 32 < a.tokens.vocab; i += kCluster * kSortThreads) a.named[i] = 0;
         cluster.sync();
     }
     bool bad = false;
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");        // this CTA's shared memory may be written
     for (int pass = 0; pass < a.passes; ++pass) {
-        const int shift = pass * kDigitBits;
+        const int shift = pass * a.bits;
         uint2* out = (a.passes - 1 - pass) & 1 ? a.pairs[1] : a.pairs[0];
         const uint2* in = (a.passes - 1 - pass) & 1 ? a.pairs[0] : a.pairs[1];
         const auto load = [&](unsigned i) {
@@ -386,20 +402,46 @@ embedding_sort_kernel(SortArguments a) {
             const long long token = a.tokens.at(i, bad);
             return make_uint2(static_cast<unsigned>(token < 0 ? a.tokens.vocab : token), i);
         };
-        const Head head = load_head(first, last, load);
-        for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) counts[i] = 0;
-        __syncthreads();
-        walk(first, last, head, load, [&](bool here, uint2 pair) {
-            const unsigned digit = (pair.x >> shift) & (kDigits - 1), same = same_digit(here, digit);
-            if (here && (same & below_lane) == 0) mine[digit] += __popc(same);
-            if (kClear && pass == 0 && here && a.named != nullptr && pair.x < a.tokens.vocab)
+        const auto digit_of = [&](uint2 pair) { return (pair.x >> shift) & static_cast<unsigned>(digits - 1); };
+        const auto name = [&](bool here, uint2 pair) {
+            if (pass == 0 && here && a.named != nullptr && pair.x < a.tokens.vocab)
                 atomicOr(a.named + (pair.x >> 5), 1u << (pair.x & 31u));
-            __syncwarp();
-        });
+        };
+        const Head<kSteps> head = load_head<kSteps>(first, last, load);
+        for (int i = threadIdx.x; i < kSortWarps << a.bits; i += kSortThreads)
+            counts[(i >> a.bits) * kDigits + (i & (digits - 1))] = 0;
         __syncthreads();
-        if (threadIdx.x < kDigits) {
+        unsigned places[kSteps];                             // in the warp's share of the digit
+        if (held) {
+            unsigned same[kSteps];
+            #pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                if (first + s * 32 >= last) break;
+                same[s] = same_digit(first + s * 32 + lane < last, digit_of(head.pairs[s]), a.bits);
+            }
+            #pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                if (first + s * 32 >= last) break;
+                const bool here = first + s * 32 + lane < last;
+                const unsigned digit = digit_of(head.pairs[s]), before = same[s] & below_lane, there = mine[digit];
+                places[s] = there + __popc(before);
+                __syncwarp();
+                if (here && before == 0) mine[digit] = there + __popc(same[s]);
+                __syncwarp();
+                name(here, head.pairs[s]);
+            }
+        } else {
+            walk<kSteps>(first, last, head, load, [&](bool here, uint2 pair) {
+                const unsigned digit = digit_of(pair), same = same_digit(here, digit, a.bits);
+                if (here && (same & below_lane) == 0) mine[digit] += __popc(same);
+                name(here, pair);
+                __syncwarp();
+            });
+        }
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < digits) {
             unsigned sum = 0;
-            #pragma unroll 8
+            #pragma unroll 16
             for (int w = 0; w < kSortWarps; ++w) {
                 const unsigned n = counts[w * kDigits + threadIdx.x];
                 counts[w * kDigits + threadIdx.x] = sum;
@@ -407,13 +449,20 @@ embedding_sort_kernel(SortArguments a) {
             }
             totals[threadIdx.x] = sum;
         }
+        if (pass == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        __syncthreads();
+        for (int i = threadIdx.x; i < kCluster << (a.bits - 2); i += kSortThreads) {
+            const int quad = i & (digits / 4 - 1);
+            uint4* share = reinterpret_cast<uint4*>(cluster.map_shared_rank(shares + rank * kDigits, i >> (a.bits - 2)));
+            share[quad] = reinterpret_cast<const uint4*>(totals)[quad];
+        }
         cluster.sync();
         // first place of this CTA's share of each digit
         unsigned below = 0, all = 0, inclusive = 0;
-        if (threadIdx.x < kDigits) {
+        if (static_cast<int>(threadIdx.x) < digits) {
             #pragma unroll
             for (unsigned r = 0; r < kCluster; ++r) {
-                const unsigned n = *cluster.map_shared_rank(totals + threadIdx.x, r);
+                const unsigned n = shares[r * kDigits + threadIdx.x];
                 below += r < rank ? n : 0;
                 all += n;
             }
@@ -426,21 +475,32 @@ embedding_sort_kernel(SortArguments a) {
             if (lane == 31) sums[warp] = inclusive;
         }
         __syncthreads();
-        if (threadIdx.x < kDigits) {
-            for (int w = 0; w < warp; ++w) inclusive += sums[w];
+        if (static_cast<int>(threadIdx.x) < digits) {
+            inclusive += __reduce_add_sync(0xffffffffu, lane < warp ? sums[lane] : 0);
             starts[threadIdx.x] = inclusive - all + below;
         }
         __syncthreads();
-        walk(first, last, head, load, [&](bool here, uint2 pair) {
-            const unsigned digit = (pair.x >> shift) & (kDigits - 1), same = same_digit(here, digit);
-            const unsigned before = same & below_lane;
-            const unsigned place = here ? starts[digit] + mine[digit] + __popc(before) : a.count;
-            if (place < a.count) out[place] = pair;          // (it is, unless the tokens are written meanwhile)
-            __syncwarp();
-            if (here && before == 0) mine[digit] += __popc(same);
-            __syncwarp();
-        });
-        cluster.sync();                                      // the pass is in memory, and nobody reads these totals
+        if (held) {
+            #pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                const bool here = first + s * 32 + lane < last;
+                const unsigned digit = digit_of(head.pairs[s]);
+                const unsigned place = here ? starts[digit] + mine[digit] + places[s] : a.count;
+                if (place < a.count) out[place] = head.pairs[s];         // (it is, unless the tokens are written meanwhile)
+            }
+        } else {
+            walk<kSteps>(first, last, head, load, [&](bool here, uint2 pair) {
+                const unsigned digit = digit_of(pair), same = same_digit(here, digit, a.bits);
+                const unsigned before = same & below_lane;
+                const unsigned place = here ? starts[digit] + mine[digit] + __popc(before) : a.count;
+                if (place < a.count) out[place] = pair;
+                __syncwarp();
+                if (here && before == 0) mine[digit] += __popc(same);
+                __syncwarp();
+            });
+        }
+        // the pass is in memory, and nobody reads these shares (the last pass writes no more of them)
+        if (pass + 1 < a.passes) cluster.sync();
     }
     if (bad && a.status != nullptr) atomicExch(a.status, 1);
 }
@@ -852,32 +912,34 @@ GradientScratch gradient_scratch(long long count, long long vocab, int width) {
 
 using SortKernel = void (*)(SortArguments);
 
-cudaLaunchConfig_t cluster_launch(int cluster, long long ctas, cudaLaunchAttribute& attribute, cudaStream_t stream) {
+cudaLaunchConfig_t cluster_launch(int cluster, long long ctas, int shared, cudaLaunchAttribute& attribute, cudaStream_t stream) {
     attribute.id = cudaLaunchAttributeClusterDimension;
     attribute.val.clusterDim.x = cluster;
     attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(static_cast<unsigned>(ctas));
     config.blockDim = dim3(kSortThreads);
-    config.dynamicSmemBytes = kSortShared;
+    config.dynamicSmemBytes = shared;
     config.stream = stream;
     config.attrs = &attribute;
     config.numAttrs = 1;
     return config;
 }
 
+// The sorting cluster, and as many more as `pieces` CTAs take.
 template <int kCluster>
-cudaError_t launch_cluster(SortKernel kernel, long long ctas, const SortArguments& a, cudaStream_t stream) {
+cudaError_t launch_cluster(SortKernel kernel, long long pieces, const SortArguments& a, cudaStream_t stream) {
     // the limit belongs to the device's context; setting it costs a fraction of a launch
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortShared);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sort_shared<kCluster>());
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attribute{};
-    const cudaLaunchConfig_t config = cluster_launch(kCluster, ctas, attribute, stream);
+    const long long ctas = kCluster + (pieces + kCluster - 1) / kCluster * kCluster;
+    const cudaLaunchConfig_t config = cluster_launch(kCluster, ctas, sort_shared<kCluster>(), attribute, stream);
     return cudaLaunchKernelEx(&config, kernel, a);
 }
 
 // Whether the current device runs clusters of 16 such CTAs: asked once per
-// device, after which the kernel may be launched so.
+// device, after which the kernels may be launched so.
 bool large_clusters() {
     constexpr int kDevices = 64;
     static std::atomic<int> known[kDevices];     // 0: not asked yet, 1: no, 2: yes
@@ -885,13 +947,16 @@ bool large_clusters() {
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kDevices) return false;
     int answer = known[device].load(std::memory_order_relaxed);
     if (answer == 0) {
-        SortKernel kernel = embedding_sort_kernel<kClusterLarge, false>;
-        cudaLaunchAttribute attribute{};
-        const cudaLaunchConfig_t config = cluster_launch(kClusterLarge, kClusterLarge, attribute, nullptr);
-        int clusters = 0;
-        const bool can = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortShared) == cudaSuccess &&
-                         cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
-                         cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) == cudaSuccess && clusters > 0;
+        const auto can_run = [](SortKernel kernel) {
+            constexpr int kShared = sort_shared<kClusterLarge>();
+            cudaLaunchAttribute attribute{};
+            const cudaLaunchConfig_t config = cluster_launch(kClusterLarge, kClusterLarge, kShared, attribute, nullptr);
+            int clusters = 0;
+            return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared) == cudaSuccess &&
+                   cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                   cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) == cudaSuccess && clusters > 0;
+        };
+        const bool can = can_run(embedding_sort_kernel<kClusterLarge, 4, 1>) && can_run(embedding_sort_kernel<kClusterLarge, 8, 1>);
         if (!can) cudaGetLastError();
         answer = can ? 2 : 1;
         known[device].store(answer, std::memory_order_relaxed);
@@ -900,9 +965,11 @@ bool large_clusters() {
 }
 
 cudaError_t launch_sort(SortArguments a, cudaStream_t stream) {
-    const long long pieces = (a.clear_bytes + kClearBytes - 1) / kClearBytes;
+    const bool small = a.count <= kSmallSort, two_ctas = !small && a.clear_bytes >= kClearLong + kClearToken * a.count;
+    a.clear_piece = small || two_ctas ? kClearPiece : 2 * kClearPiece;
+    const long long pieces = (a.clear_bytes + a.clear_piece - 1) / a.clear_piece;
     if (pieces > 2147483000ll) return cudaErrorInvalidValue;
-    if (a.count <= kSmallSort) {
+    if (small) {
         int padded = 64;
         while (padded < static_cast<int>(a.count)) padded <<= 1;
         const unsigned ctas = static_cast<unsigned>(1 + pieces);
@@ -912,15 +979,17 @@ cudaError_t launch_sort(SortArguments a, cudaStream_t stream) {
             embedding_small_sort_kernel<unsigned long long><<<ctas, kSortThreads, 0, stream>>>(a, padded);
         return cudaPeekAtLastError();
     }
-    a.passes = 1;                                // over the bits of the largest key, `vocab`
-    while (a.tokens.vocab >> (kDigitBits * a.passes) != 0) ++a.passes;
-    if (pieces > 0) {
-        const long long ctas = kClusterSmall + (pieces + kClusterSmall - 1) / kClusterSmall * kClusterSmall;
-        return launch_cluster<kClusterSmall>(embedding_sort_kernel<kClusterSmall, true>, ctas, a, stream);
-    }
-    if (a.count > kClusterSmall * kSortThreads * kSteps && large_clusters())
-        return launch_cluster<kClusterLarge>(embedding_sort_kernel<kClusterLarge, false>, kClusterLarge, a, stream);
-    return launch_cluster<kClusterSmall>(embedding_sort_kernel<kClusterSmall, false>, kClusterSmall, a, stream);
+    int bits = 1;                                // of the largest key, `vocab`
+    while (a.tokens.vocab >> bits != 0) ++bits;
+    a.passes = (bits + kDigitBits - 1) / kDigitBits;
+    a.bits = (bits + a.passes - 1) / a.passes;
+    if (a.bits < kLeastBits) a.bits = kLeastBits;
+    if (two_ctas) return launch_cluster<kClusterSmall>(embedding_sort_kernel<kClusterSmall, 4, 2>, pieces, a, stream);
+    if (a.count <= kClusterSmall * kSortThreads * 4 || !large_clusters())
+        return launch_cluster<kClusterSmall>(embedding_sort_kernel<kClusterSmall, 4, 1>, pieces, a, stream);
+    return launch_cluster<kClusterLarge>(a.count > kClusterLarge * kSortThreads * 4 ? embedding_sort_kernel<kClusterLarge, 8, 1>
+                                                                                    : embedding_sort_kernel<kClusterLarge, 4, 1>,
+                                         pieces, a, stream);
 }
 
 template <typename G, typename T, bool kVector, bool kAdd>
