@@ -14,7 +14,7 @@
 //
 //   sort    pairs (row, position).  Up to 2048 tokens: one CTA, a bitonic sort
 //           in shared memory.  More: one cluster of CTAs, a stable radix sort
-//           of 9 bits a pass, digit counts exchanged through distributed shared
+//           of up to 9 bits a pass, digit counts exchanged through distributed shared
 //           memory, the cluster's barriers between the passes.  (When the whole
 //           table is written, the other SMs write its zeros in the same launch:
 //           they are most of the traffic and take longer than the sort, whose
@@ -184,13 +184,16 @@ embedding_lookup_kernel(LookupArguments a) {
 constexpr int kSmallBits = 11, kSmallSort = 1 << kSmallBits;   // tokens that one CTA sorts
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 // CTAs of the sorting cluster: 8 is the portable size.  16, where the device has
-// them, for more tokens than 8 CTAs hold in their registers and no long clearing
-// beside the sort to hide it (65536 tokens added to a table: 76 us with 8, 65 us with 16).
+// them, for more tokens than one for each thread of 8 (20000 tokens added to a
+// table: 33 us with 8, 31 us with 16; 65536: 74 and 64 us), or beside zeros, which
+// clusters of 16 write more slowly, than 8 hold in their registers (30000 tokens
+// and 307 MB of zeros: 98 us with 8, 105 us with 16).
 constexpr int kClusterSmall = 8, kClusterLarge = 16;
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;   // of a pass at most
 constexpr int kLeastBits = 5;                   // a warp of digits
-template <int kCluster>
-constexpr int sort_shared() { return (kSortWarps + 2 + kCluster) * kDigits * 4; }
+// Bytes of shared memory; with one CTA of an SM there is room for masks beside the counts.
+template <int kCluster, int kResident>
+constexpr int sort_shared() { return (kSortWarps * (kResident == 1 ? 2 : 1) + 2 + kCluster) * kDigits * 4; }
 // Zeros of a CTA beside the sort; and from how many bytes on, these and some for
 // each token, they take longer than the sort (8192 tokens, 197 MB: 59 us with two
 // CTAs of an SM, 61 us with one; 30000 tokens, 307 MB: 106 and 98 us; 65536
@@ -334,17 +337,33 @@ __device__ __forceinline__ void walk(unsigned from, unsigned to, Head<kSteps> he
     }
 }
 
-// Lanes that are here and have the lane's digit: a vote per bit.
-__device__ __forceinline__ unsigned same_digit(bool here, unsigned digit, int bits) {
-    unsigned same = __ballot_sync(0xffffffffu, here);
-    #pragma unroll
-    for (int b = 0; b < kDigitBits; ++b) {
-        if (b >= bits) break;
-        const bool set = (digit >> b) & 1u;
-        const unsigned votes = __ballot_sync(0xffffffffu, set);
-        same &= set ? votes : ~votes;
+// Lanes that are here and have the lane's digit (of a lane that is not here:
+// anything).  With masks, a zero for each digit of the warp's: every lane sets its
+// bit, and the first of a digit leaves a zero again; the caller's next __syncwarp()
+// ends that.  Without: a vote per bit.  (Votes, of which an SM finishes one in some
+// 4 clocks, were what ranking waited for: 131072 tokens of 128 columns added 63 us
+// with them, 60 us with masks; a match instruction is no faster than the votes.)
+template <bool kMasks>
+__device__ __forceinline__ unsigned same_digit(bool here, unsigned digit, int bits, unsigned* masks) {
+    if constexpr (kMasks) {
+        const unsigned lane = threadIdx.x & 31;
+        if (here) atomicOr(masks + digit, 1u << lane);
+        __syncwarp();
+        const unsigned same = masks[digit];
+        __syncwarp();
+        if (here && (same & ((1u << lane) - 1u)) == 0) masks[digit] = 0;
+        return same;
+    } else {
+        unsigned same = __ballot_sync(0xffffffffu, here);
+        #pragma unroll
+        for (int b = 0; b < kDigitBits; ++b) {
+            if (b >= bits) break;
+            const bool set = (digit >> b) & 1u;
+            const unsigned votes = __ballot_sync(0xffffffffu, set);
+            same &= set ? votes : ~votes;
+        }
+        return same;
     }
-    return same;
 }
 
 // Stable: warps own consecutive stretches of the input, a warp walks its
@@ -367,6 +386,8 @@ embedding_sort_kernel(SortArguments a) {
     unsigned* totals = shared + kSortWarps * kDigits;        // [digits]
     unsigned* starts = totals + kDigits;                     // [digits]
     unsigned* shares = starts + kDigits;                     // [CTAs][digits]: the totals of each
+    constexpr bool kMasks = kResident == 1;
+    unsigned* masks = shares + kCluster * kDigits + (kMasks ? (threadIdx.x >> 5) * kDigits : 0);
     __shared__ unsigned sums[32];
     let_next_start();
     if (blockIdx.x >= kCluster) {                            // whole clusters of them: no barrier is shared
@@ -391,6 +412,8 @@ embedding_sort_kernel(SortArguments a) {
         for (long long i = rank * kSortThreads + threadIdx.x; i * 32 < a.tokens.vocab; i += kCluster * kSortThreads) a.named[i] = 0;
         cluster.sync();
     }
+    if (kMasks)
+        for (int i = lane; i < digits; i += 32) masks[i] = 0;
     bool bad = false;
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");        // this CTA's shared memory may be written
     for (int pass = 0; pass < a.passes; ++pass) {
@@ -413,26 +436,20 @@ embedding_sort_kernel(SortArguments a) {
         __syncthreads();
         unsigned places[kSteps];                             // in the warp's share of the digit
         if (held) {
-            unsigned same[kSteps];
-            #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                if (first + s * 32 >= last) break;
-                same[s] = same_digit(first + s * 32 + lane < last, digit_of(head.pairs[s]), a.bits);
-            }
             #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 if (first + s * 32 >= last) break;
                 const bool here = first + s * 32 + lane < last;
-                const unsigned digit = digit_of(head.pairs[s]), before = same[s] & below_lane, there = mine[digit];
+                const unsigned digit = digit_of(head.pairs[s]), there = mine[digit];
+                const unsigned same = same_digit<kMasks>(here, digit, a.bits, masks), before = same & below_lane;
                 places[s] = there + __popc(before);
-                __syncwarp();
-                if (here && before == 0) mine[digit] = there + __popc(same[s]);
+                if (here && before == 0) mine[digit] = there + __popc(same);
                 __syncwarp();
                 name(here, head.pairs[s]);
             }
         } else {
             walk<kSteps>(first, last, head, load, [&](bool here, uint2 pair) {
-                const unsigned digit = digit_of(pair), same = same_digit(here, digit, a.bits);
+                const unsigned digit = digit_of(pair), same = same_digit<kMasks>(here, digit, a.bits, masks);
                 if (here && (same & below_lane) == 0) mine[digit] += __popc(same);
                 name(here, pair);
                 __syncwarp();
@@ -490,11 +507,11 @@ embedding_sort_kernel(SortArguments a) {
             }
         } else {
             walk<kSteps>(first, last, head, load, [&](bool here, uint2 pair) {
-                const unsigned digit = digit_of(pair), same = same_digit(here, digit, a.bits);
+                const unsigned digit = digit_of(pair), same = same_digit<kMasks>(here, digit, a.bits, masks);
                 const unsigned before = same & below_lane;
                 const unsigned place = here ? starts[digit] + mine[digit] + __popc(before) : a.count;
                 if (place < a.count) out[place] = pair;
-                __syncwarp();
+                __syncwarp();                                // everyone has read its place
                 if (here && before == 0) mine[digit] += __popc(same);
                 __syncwarp();
             });
@@ -927,14 +944,14 @@ cudaLaunchConfig_t cluster_launch(int cluster, long long ctas, int shared, cudaL
 }
 
 // The sorting cluster, and as many more as `pieces` CTAs take.
-template <int kCluster>
+template <int kCluster, int kResident>
 cudaError_t launch_cluster(SortKernel kernel, long long pieces, const SortArguments& a, cudaStream_t stream) {
     // the limit belongs to the device's context; setting it costs a fraction of a launch
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sort_shared<kCluster>());
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sort_shared<kCluster, kResident>());
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attribute{};
     const long long ctas = kCluster + (pieces + kCluster - 1) / kCluster * kCluster;
-    const cudaLaunchConfig_t config = cluster_launch(kCluster, ctas, sort_shared<kCluster>(), attribute, stream);
+    const cudaLaunchConfig_t config = cluster_launch(kCluster, ctas, sort_shared<kCluster, kResident>(), attribute, stream);
     return cudaLaunchKernelEx(&config, kernel, a);
 }
 
@@ -948,7 +965,7 @@ bool large_clusters() {
     int answer = known[device].load(std::memory_order_relaxed);
     if (answer == 0) {
         const auto can_run = [](SortKernel kernel) {
-            constexpr int kShared = sort_shared<kClusterLarge>();
+            constexpr int kShared = sort_shared<kClusterLarge, 1>();
             cudaLaunchAttribute attribute{};
             const cudaLaunchConfig_t config = cluster_launch(kClusterLarge, kClusterLarge, kShared, attribute, nullptr);
             int clusters = 0;
@@ -984,10 +1001,10 @@ cudaError_t launch_sort(SortArguments a, cudaStream_t stream) {
     a.passes = (bits + kDigitBits - 1) / kDigitBits;
     a.bits = (bits + a.passes - 1) / a.passes;
     if (a.bits < kLeastBits) a.bits = kLeastBits;
-    if (two_ctas) return launch_cluster<kClusterSmall>(embedding_sort_kernel<kClusterSmall, 4, 2>, pieces, a, stream);
-    if (a.count <= kClusterSmall * kSortThreads * 4 || !large_clusters())
-        return launch_cluster<kClusterSmall>(embedding_sort_kernel<kClusterSmall, 4, 1>, pieces, a, stream);
-    return launch_cluster<kClusterLarge>(a.count > kClusterLarge * kSortThreads * 4 ? embedding_sort_kernel<kClusterLarge, 8, 1>
+    if (two_ctas) return launch_cluster<kClusterSmall, 2>(embedding_sort_kernel<kClusterSmall, 4, 2>, pieces, a, stream);
+    if (a.count <= kClusterSmall * kSortThreads * (pieces > 0 ? 4 : 1) || !large_clusters())
+        return launch_cluster<kClusterSmall, 1>(embedding_sort_kernel<kClusterSmall, 4, 1>, pieces, a, stream);
+    return launch_cluster<kClusterLarge, 1>(a.count > kClusterLarge * kSortThreads * 4 ? embedding_sort_kernel<kClusterLarge, 8, 1>
                                                                                     : embedding_sort_kernel<kClusterLarge, 4, 1>,
                                          pieces, a, stream);
 }
