@@ -217,6 +217,39 @@ def test_small_sorts(cuda, vocab, count):
     check_gradient(tokens, dout, whole, 1.0, vocab)
 
 
+@pytest.mark.parametrize("law", ("even", "text"))
+@pytest.mark.parametrize("count", (8192, 8193, 32768, 32769, 65536, 65537, 131072, 131073, 300001))
+def test_sorts_of_several_ctas(cuda, count, law):
+    """The cluster's sizes, and stretches that fill a warp's registers, pass them and pass them twice."""
+    rng = np.random.default_rng(count)
+    vocab = 900
+    tokens = some_tokens(rng, count, vocab, 0.03, law)
+    dout = dev(rng.standard_normal((count, 4)).astype(np.float32))
+    before = torch.ones(vocab, 4, device="cuda")
+    added, whole = before.clone(), torch.full((vocab, 4), 9.0, device="cuda")
+    TokenEmbedding.gradient(0, dev(tokens), dout, added, accumulate=True)
+    TokenEmbedding.gradient(0, dev(tokens), dout, whole)
+    torch.cuda.synchronize()
+    check_gradient(tokens, dout, added, 1.0, vocab, before)
+    check_gradient(tokens, dout, whole, 1.0, vocab)
+
+
+@pytest.mark.parametrize("count,vocab,width", ((3000, 70000, 1024), (8192, 64000, 1024), (30000, 100_000, 1024),
+                                               (140_000, 340_000, 1024)))
+def test_zeros_beside_the_sort(cuda, count, vocab, width):
+    """The sums do not depend on how the sort and the zeros share the machine: the bits of a gradient added to zeros."""
+    generator = torch.Generator(device="cuda").manual_seed(count)
+    tokens = torch.randint(-1, vocab, (count,), generator=generator, device="cuda")
+    tokens[::7] = tokens[0]                              # one that crosses every chunk of its own
+    dout = torch.randn(count, width, generator=generator, device="cuda", dtype=torch.bfloat16)
+    whole, added = torch.full((vocab, width), 9.0, device="cuda"), torch.zeros(vocab, width, device="cuda")
+    TokenEmbedding.gradient(0, tokens, dout, whole)
+    TokenEmbedding.gradient(0, tokens, dout, added, accumulate=True)
+    torch.cuda.synchronize()
+    assert torch.equal(whole, added)
+    assert not whole[~torch.zeros(vocab, dtype=torch.bool, device="cuda").index_fill_(0, tokens[tokens >= 0], True)].any()
+
+
 @pytest.mark.parametrize("vocab,width", ((70000, 4), (300_000, 4), (1 << 28, 1)))
 def test_one_bucket_takes_all(cuda, vocab, width):
     """Rows that agree in their low 9 bits: one, two and three passes over the others."""
