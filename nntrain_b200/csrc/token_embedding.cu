@@ -537,8 +537,10 @@ __host__ __device__ constexpr int lane_values() { return kVector && sizeof(G) ==
 struct RowsArguments {
     const uint2* pairs;                // sorted (row, position)
     unsigned* crossing;                // tokens that cross chunks: number of short and of long ones, then
-    uint2* crossing_short;             // the chunks in which they begin, and their rows
-    uint2* crossing_long;
+    unsigned* crossing_short;          // the chunks in which they begin
+    unsigned* crossing_long;
+    unsigned* rows_short;              // and their rows, where the sort's second array was
+    unsigned* rows_long;
     float* tails;                      // [chunk][width]: sum up to the chunk's end of a token that goes on
     float* heads;                      // [chunk][width]: rest of a token that began in an earlier chunk
     const void* gradient;              // dout
@@ -724,7 +726,9 @@ embedding_rows_kernel(RowsArguments a) {
                 if (!begun_before && first == 0 && lane == 0) {
                     const unsigned long long far = static_cast<unsigned long long>(chunk + kLongChunks) * size;
                     const bool is_long = far < a.count && a.pairs[far].x == here;
-                    (is_long ? a.crossing_long : a.crossing_short)[atomicAdd(a.crossing + is_long, 1u)] = make_uint2(chunk, here);
+                    const unsigned place = atomicAdd(a.crossing + is_long, 1u);
+                    (is_long ? a.crossing_long : a.crossing_short)[place] = chunk;
+                    (is_long ? a.rows_long : a.rows_short)[place] = here;
                 }
             } else if (begun_before) {
                 store_partial<kValues, kVector>(a.heads, chunk, a.width, first, lane, sum);
@@ -803,16 +807,21 @@ embedding_join_kernel(RowsArguments a) {
         zero_rows<T>(a, a.join_groups + blockIdx.x - a.join_ctas);
         return;
     }
-    const uint2* list = is_long ? a.crossing_long : a.crossing_short;
+    const unsigned* list = is_long ? a.crossing_long : a.crossing_short;
+    const unsigned* rows = is_long ? a.rows_long : a.rows_short;
     const unsigned long long step = is_long ? a.long_ctas : static_cast<unsigned long long>(a.join_ctas - a.long_ctas) * kWarpsPerCta;
     unsigned long long task = is_long ? blockIdx.x : static_cast<unsigned long long>(blockIdx.x - a.long_ctas) * kWarpsPerCta + warp;
     // (the first entry is loaded beside the number of them, from a place that the list has)
-    const unsigned long long places = is_long ? a.chunks / kLongChunks + 1 : a.chunks, place = task / a.slices;
-    uint2 token = list[place < places ? place : 0];
+    const unsigned long long places = is_long ? a.chunks / kLongChunks + 1 : a.chunks;
+    unsigned long long place = task / a.slices < places ? task / a.slices : 0;
+    unsigned begin = list[place], key = rows[place];
     const unsigned long long tasks = static_cast<unsigned long long>(a.crossing[is_long]) * a.slices;
     for (; task < tasks; task += step) {
-        if (task >= step) token = list[task / a.slices];
-        const unsigned begin = token.x, key = token.y;
+        if (task >= step) {
+            place = task / a.slices;
+            begin = list[place];
+            key = rows[place];
+        }
         const int first = static_cast<int>(task % a.slices) * (kValues * 32);
         const unsigned end = last_chunk_of(a, key, begin, lane), parts = end - begin + 1;
         float sum[kValues] = {}, old[kAdd ? kValues : 1];
@@ -920,8 +929,8 @@ GradientScratch gradient_scratch(long long count, long long vocab, int width) {
     for (int i = 0; i < 2; ++i) s.pairs[i] = take(count * 8);
     s.named = take((vocab + 31) / 32 * 4);
     s.crossing = take(8);
-    s.crossing_short = take(s.chunks * 8);
-    s.crossing_long = take((s.chunks / kLongChunks + 1) * 8);
+    s.crossing_short = take(s.chunks * 4);
+    s.crossing_long = take((s.chunks / kLongChunks + 1) * 4);
     s.tails = take(s.chunks * width * 4);
     s.heads = take(s.chunks * width * 4);
     return s;
@@ -1069,8 +1078,10 @@ int gradient(int device, int gradient_kind, const void* out_gradient, long long 
     RowsArguments a{};
     a.pairs = sort.pairs[0];
     a.crossing = sort.crossing;
-    a.crossing_short = reinterpret_cast<uint2*>(scratch + s.crossing_short);
-    a.crossing_long = reinterpret_cast<uint2*>(scratch + s.crossing_long);
+    a.crossing_short = reinterpret_cast<unsigned*>(scratch + s.crossing_short);
+    a.crossing_long = reinterpret_cast<unsigned*>(scratch + s.crossing_long);
+    a.rows_short = reinterpret_cast<unsigned*>(scratch + s.pairs[1]);    // chunks + chunks / 16 + 1 of them: less than pairs
+    a.rows_long = a.rows_short + s.chunks;
     a.tails = reinterpret_cast<float*>(scratch + s.tails);
     a.heads = reinterpret_cast<float*>(scratch + s.heads);
     a.gradient = out_gradient;

@@ -409,3 +409,22 @@ def test_refusals(cuda):
         TokenEmbedding.gradient(0, tokens, out, table, workspace=torch.zeros(16, dtype=torch.uint8, device="cuda"))
     with pytest.raises(ValueError, match="token_status"):
         TokenEmbedding.lookup(0, tokens, table, out, token_status=torch.zeros(1, device="cuda"))
+
+
+@pytest.mark.parametrize("count", (3000, 20000, 70000))
+def test_recorded_sorts_of_several_ctas(cuda, count):
+    """A cluster's sort in a graph, replayed on other tokens than it was recorded with."""
+    rng = np.random.default_rng(count)
+    vocab, width = 5000, 40
+    dout = dev(rng.standard_normal((count, width)).astype(np.float32))
+    tokens, got = torch.zeros(count, dtype=torch.int64, device="cuda"), torch.zeros(vocab, width, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        TokenEmbedding.gradient(0, tokens, dout, got, scale=0.5, accumulate=True)
+    for law in ("text", "even"):
+        other = some_tokens(rng, count, vocab, 0.1, law)
+        tokens.copy_(torch.from_numpy(other))
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_gradient(other, dout, got, 0.5, vocab)
