@@ -47,9 +47,10 @@ typedef struct nntrain_native_error_info {
  * reference, which passes one tensor per call).  kind: 0 = fp32, 1 = bf16,
  * 2 = BFP8.  values: the tensor, or its payload.  scales, block_size: of a
  * BFP8 tensor (block_size 0 = one scale).  destination: where the clipped
- * values (of a BFP8 tensor: the clipped scales) go, NULL = in place; it may
- * not overlap `values` in part.  Addresses need the alignment of their type
- * only.  first_chunk is filled in by nntrain_gradient_list_plan. */
+ * values (of a BFP8 tensor: the clipped scales) go, NULL = in place; it may be
+ * `values` (of a BFP8 tensor: `scales`) itself and not overlap either in any
+ * other way.  Addresses need the alignment of their type only.  first_chunk is
+ * filled in by nntrain_gradient_list_plan. */
 typedef struct nntrain_gradient_tensor {
     const void* values;
     float* scales;

@@ -466,29 +466,32 @@ bool valid_tensor(const nntrain_gradient_tensor& t) {
 struct Range {
     std::uintptr_t begin, end;
     int tensor;
+    bool source;                        // read: what its own tensor's clip is made from
 };
 
 // Whether what the clip writes for one tensor is read or written for another
 // one (the same tensor twice, a destination over a neighbour): chunks run in any
-// order, so such a list has no defined result.
+// order, so such a list has no defined result.  In place a tensor's values, or a
+// payload's scales, are read and written at one place by one thread; scales are
+// never written over a payload, which may be just as long.
 bool overlapping(const nntrain_gradient_tensor* tensors, int count) {
     std::vector<Range> written, read;
     for (int i = 0; i < count; ++i) {
         const nntrain_gradient_tensor& t = tensors[i];
         if (t.length == 0) continue;
-        const auto range = [&](const void* p, long long bytes) {
+        const auto range = [&](const void* p, long long bytes, bool source) {
             const std::uintptr_t at = reinterpret_cast<std::uintptr_t>(p);
-            return Range{at, at + static_cast<std::uintptr_t>(bytes), i};
+            return Range{at, at + static_cast<std::uintptr_t>(bytes), i, source};
         };
         if (t.kind == kKindBfp8) {
             const long long blocks = t.block_size == 0 || t.block_size >= t.length ? 1 : (t.length + t.block_size - 1) / t.block_size;
-            read.push_back(range(t.values, t.length));
-            read.push_back(range(t.scales, blocks * 4));
-            written.push_back(range(t.destination != nullptr ? t.destination : t.scales, blocks * 4));
+            read.push_back(range(t.values, t.length, false));
+            read.push_back(range(t.scales, blocks * 4, true));
+            written.push_back(range(t.destination != nullptr ? t.destination : t.scales, blocks * 4, false));
         } else {
             const long long bytes = t.length * (t.kind == kKindF32 ? 4 : 2);
-            read.push_back(range(t.values, bytes));
-            written.push_back(range(t.destination != nullptr ? t.destination : t.values, bytes));
+            read.push_back(range(t.values, bytes, true));
+            written.push_back(range(t.destination != nullptr ? t.destination : t.values, bytes, false));
         }
     }
     const auto by_begin = [](const Range& a, const Range& b) { return a.begin < b.begin; };
@@ -500,7 +503,7 @@ bool overlapping(const nntrain_gradient_tensor* tensors, int count) {
         auto w = std::upper_bound(written.begin(), written.end(), r, by_begin);
         if (w != written.begin()) --w;
         for (; w != written.end() && w->begin < r.end; ++w) {
-            const bool itself = w->tensor == r.tensor && w->begin == r.begin && w->end == r.end;
+            const bool itself = r.source && w->tensor == r.tensor && w->begin == r.begin && w->end == r.end;
             if (w->end > r.begin && !itself) return true;
         }
     }

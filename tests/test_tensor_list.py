@@ -115,6 +115,21 @@ def test_plan_refuses_tensors_that_share_what_is_written(lib):
     assert plan(lib, empty)[0] == 0
 
 
+@pytest.mark.parametrize("length,block", ((64, 4), (4, 0), (4, 8), (8, 4), (64, 32)))
+def test_plan_refuses_scales_written_over_their_own_payload(lib, length, block):
+    """Blocks of four values have as many bytes of scales as of codes: the two ranges are then the same one."""
+    table = table_of([length], kind=2, block=block)
+    table["values"], table["scales"] = 0x1000, 0x2000
+    assert plan(lib, table)[0] == 0
+    for destination, status in ((0x2000, 0), (0x1000 + length, 0), (0x1000, INVALID)):
+        table["destination"] = destination
+        assert plan(lib, table)[0] == status, hex(destination)
+    table["scales"], table["destination"] = 0x1000, 0
+    assert plan(lib, table)[0] == INVALID                           # in place, scales where the payload is
+    table["destination"] = 0x3000
+    assert plan(lib, table)[0] == 0                                 # both are only read
+
+
 def test_clip_refusals_come_before_the_device(lib):
     def call(tensors=4096, count=1, chunk_map=4096, chunks=1, values=4096, workspace=4096, max_norm=1.0, out=4096):
         return lib.nntrain_gradient_list_clip(0, tensors, count, chunk_map, chunks, values, workspace, max_norm, 1, out,
