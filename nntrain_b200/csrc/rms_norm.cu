@@ -36,6 +36,7 @@ namespace ngb {
 namespace {
 
 constexpr int kRowThreads = 512;              // most threads on a row held in registers
+constexpr int kStagedThreads = 256;           // and on one that is staged in shared memory
 constexpr int kLoopThreads = 256;             // threads on a row that is not
 constexpr int kMostPartials = 1184;           // most CTAs that leave a partial weight gradient: 8 on each of 148 SMs
 constexpr int kJoinColumns = 8, kJoinRows = 64;   // 32 bytes of a partial, a sector
@@ -683,7 +684,8 @@ int resident_grid(int threads, int shared, long long rows) {
     std::atomic<int>& slot = known[threads / 32];
     int fit = slot.load(std::memory_order_relaxed);
     if (fit == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kKernel, threads, shared) != cudaSuccess || fit < 1) fit = 1;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kKernel, threads, shared) != cudaSuccess || fit < 1)
+            return grid_for(rows, 1);            // not kept: the next call asks again
         slot.store(fit, std::memory_order_relaxed);
     }
     return grid_for(rows, fit);
@@ -706,24 +708,30 @@ RowShape row_shape(int units, long long rows) {
     const bool wide = sizeof(T) == 2 && units > 64 && rows >= sm_count();
     for (int groups = wide ? 2 : 1; groups <= 4; groups *= 2) {
         const int threads = threads_for(units, groups);
-        if (threads <= 256 || (groups == 4 && threads <= kRowThreads)) return {groups, threads};
+        if (threads <= kStagedThreads || (groups == 4 && threads <= kRowThreads)) return {groups, threads};
     }
     return {0, 0};
 }
 
-// Rows that are staged have at most 256 threads, so at most 48 KB in flight: with
-// the reduction's slots a little more than a launch may ask for by itself.
-template <auto kKernel>
-cudaError_t allow_shared(int shared) {
-    return shared < (40 << 10) ? cudaSuccess
-                               : cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+// A staged row's kStagedThreads threads have at most 48 KB in flight: with the
+// reduction's slots a little more than a launch may ask for by itself.  The limit
+// belongs to the kernel on the device, not to a launch, so it is always set to the
+// most that the kernel can ask for: set to each launch's own size, it made the
+// launches of another host thread with a wider row fail.
+template <auto kKernel, int kThreadBytes>
+cudaError_t allow_shared() {
+    constexpr int kMost = kStagedThreads * kThreadBytes;
+    if constexpr (kMost < (40 << 10)) return cudaSuccess;
+    else return cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
 }
 
 template <typename T, int kVec, int kGroups, int kBlock>
 cudaError_t launch_forward(const ForwardArguments& a, int threads, cudaStream_t stream) {
     constexpr auto kKernel = rms_norm_forward_kernel<T, kVec, kGroups, kBlock>;
-    const int shared = threads * RowRing<T, kVec, kGroups, 2>::kThreadBytes;
-    const cudaError_t e = allow_shared<kKernel>(shared);
+    constexpr int kThreadBytes = RowRing<T, kVec, kGroups, 2>::kThreadBytes;
+    static_assert(kThreadBytes == 0 || kGroups < 4, "four groups a thread may have kRowThreads threads");
+    const int shared = threads * kThreadBytes;
+    const cudaError_t e = allow_shared<kKernel, kThreadBytes>();
     if (e != cudaSuccess) return e;
     kKernel<<<resident_grid<kKernel>(threads, shared, a.rows), threads, shared, stream>>>(a);
     return cudaPeekAtLastError();
@@ -763,8 +771,10 @@ cudaError_t run_forward(const ForwardArguments& a, bool vector_ok, cudaStream_t 
 template <typename T, int kVec, int kGroups>
 cudaError_t launch_backward(const BackwardArguments& a, int threads, int& grid, cudaStream_t stream) {
     constexpr auto kKernel = rms_norm_backward_kernel<T, kVec, kGroups>;
-    const int shared = threads * RowRing<T, kVec, kGroups, 3>::kThreadBytes;
-    const cudaError_t e = allow_shared<kKernel>(shared);
+    constexpr int kThreadBytes = RowRing<T, kVec, kGroups, 3>::kThreadBytes;
+    static_assert(kThreadBytes == 0 || kGroups < 4, "four groups a thread may have kRowThreads threads");
+    const int shared = threads * kThreadBytes;
+    const cudaError_t e = allow_shared<kKernel, kThreadBytes>();
     if (e != cudaSuccess) return e;
     grid = resident_grid<kKernel>(threads, shared, a.rows);
     if (grid > kMostPartials) grid = kMostPartials;
