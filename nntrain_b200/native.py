@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import itertools
 
 import numpy as np
 import torch
@@ -428,7 +429,10 @@ class GradientTensorList:
     clipped scales); without one it is clipped in place.  What is written for one
     tensor may not be read or written for another.  Build it once for leaves that
     stay where they are; it holds on to the tensors, and a recorded graph needs
-    it to live as long as itself."""
+    it to live as long as itself.  Otherwise it may be dropped as soon as a call
+    has returned; only a call on a stream given by its handle (or as an
+    ExternalStream, which may end before the list does) needs it until its
+    kernels have run."""
 
     _TENSOR = np.dtype([("values", np.uint64), ("scales", np.uint64), ("destination", np.uint64),
                         ("length", np.int64), ("first_chunk", np.int64), ("kind", np.int32), ("block_size", np.int32)])
@@ -485,6 +489,20 @@ class GradientTensorList:
         self.table_address = self.buffer.data_ptr()
         self.map_address = self.table_address + table.nbytes
         self._held = (list(tensors), scales, destinations)
+        self._streams = {_current_raw_stream(device)}
+
+    def _keep_for(self, stream, handle: int) -> None:
+        """Table and tensors are not handed out again before what is now on
+        `stream`, not the one the list was built on, has run: told to torch's
+        allocator once for each stream."""
+        if isinstance(stream, (int, torch.cuda.ExternalStream)):
+            return
+        if stream is None:
+            stream = torch.cuda.current_stream(self.device)
+        for t in (self.buffer, *itertools.chain(*self._held)):
+            if t is not None:
+                t.record_stream(stream)
+        self._streams.add(handle)
 
 
 class GradientNorm:
@@ -536,10 +554,12 @@ class GradientNorm:
             _require(workspace, torch.float64, "workspace", device)
             if workspace.numel() < tensors.chunks:
                 raise ValueError("workspace is too small")
+        handle = _stream_on(device, stream)
+        if handle not in tensors._streams:
+            tensors._keep_for(stream, handle)
         check("gradient_list_clip", load().nntrain_gradient_list_clip(
             device, tensors.table_address, tensors.count, tensors.map_address, tensors.chunks, tensors.chunk_values,
-            0 if workspace is None else workspace.data_ptr(), max_norm, apply, out, norms, status,
-            _stream_on(device, stream)))
+            0 if workspace is None else workspace.data_ptr(), max_norm, apply, out, norms, status, handle))
 
 
 class Bfp8GradientOptimizers:

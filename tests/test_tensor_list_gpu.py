@@ -300,3 +300,33 @@ def test_refusals(cuda):
     with pytest.raises(ValueError, match="tensor_norms"):
         GradientNorm.clip_tensors(0, plan, 1.0, out, tensor_norms=torch.zeros(0, device="cuda"))
     assert issubclass(NativeCudaError, RuntimeError)
+
+
+@pytest.mark.parametrize("current", (False, True))
+def test_a_list_may_be_dropped_while_another_stream_works_on_it(cuda, current):
+    """Neither its table nor the tensors that only it holds are handed out again before that stream has come past."""
+    side = torch.cuda.Stream()
+    rng = np.random.default_rng(11)
+    values = rng.standard_normal(5000).astype(np.float32)
+    x, to, out = dev(values), torch.zeros(5000, device="cuda"), torch.zeros(2, device="cuda")
+    plan = GradientTensorList(0, [x], destinations=[to])
+    torch.cuda.synchronize()
+    held = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (plan.buffer, x)]
+    sizes = [plan.buffer.numel(), x.numel() * 4]
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)                 # some 0.2 s
+        if current:
+            GradientNorm.clip_tensors(0, plan, 0.1, out)
+    if not current:
+        GradientNorm.clip_tensors(0, plan, 0.1, out, stream=side)
+    del plan, x
+    later = [torch.empty(size, dtype=torch.uint8, device="cuda") for size in sizes for _ in range(200)]
+    taken = [t.data_ptr() for t in later if any(a < t.data_ptr() + t.numel() and t.data_ptr() < b for a, b in held)]
+    assert not side.query(), "the other stream was too fast to show anything"
+    assert not taken
+    for t in later:
+        t.fill_(255)
+    torch.cuda.synchronize()
+    c = host(out)[1]
+    assert c < 1.0
+    assert_bits_equal(host(to), values * c, "clipped")
