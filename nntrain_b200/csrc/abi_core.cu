@@ -51,6 +51,7 @@ int select_device(int device) {
         return static_cast<int>(cudaSuccess);
     cudaError_t status = cudaSetDevice(device);
     if (status == cudaSuccess) t_selected_device = device;
+    else cudaGetLastError();                     // the status tells it; the next launch's check must not find it
     return static_cast<int>(status);
 }
 

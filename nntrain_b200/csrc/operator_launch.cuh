@@ -1,7 +1,7 @@
 // Host plumbing shared by the training operators (list norm, RMS norm, token
-// table): the caller's device is put back when an entry point returns, and
-// dependent kernels are launched so that their prologue overlaps the end of
-// the kernel in front of them.
+// table): the caller's device is put back when an entry point returns, every
+// launch answers with its own status, and dependent kernels are launched so that
+// their prologue overlaps the end of the kernel in front of them.
 #pragma once
 
 #include "common.cuh"
@@ -12,12 +12,20 @@ constexpr Operation kOpTensorList = static_cast<Operation>(219);
 constexpr Operation kOpRmsNorm = static_cast<Operation>(220);
 constexpr Operation kOpTokenEmbedding = static_cast<Operation>(221);
 
+// A failed runtime call also stays behind as the thread's last error, where the
+// next check of any library in the process takes it for its own.  Here the entry
+// point's status tells it, so it is taken away.
+inline cudaError_t reported(cudaError_t status) {
+    if (status != cudaSuccess) cudaGetLastError();
+    return status;
+}
+
 // Selects `device` for the calling thread and selects the previous one again
 // at the end of the scope.
 class DeviceScope {
 public:
     explicit DeviceScope(int device) : device_(device) {
-        if (cudaGetDevice(&previous_) != cudaSuccess) previous_ = -1;
+        if (reported(cudaGetDevice(&previous_)) != cudaSuccess) previous_ = -1;
         status_ = select_device(device);
     }
     ~DeviceScope() {
@@ -37,6 +45,27 @@ inline bool aligned_for(const void* p, std::uintptr_t bytes) {
 
 #ifdef __CUDACC__
 
+// The status is this launch's own: peeking at the last error would also find one
+// that an earlier call on this thread left there.
+template <typename... Parameters, typename... Arguments>
+cudaError_t launch_with(cudaLaunchAttribute* attributes, int count, void (*kernel)(Parameters...), dim3 grid, int threads,
+                        size_t shared, cudaStream_t stream, Arguments... arguments) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(static_cast<unsigned>(threads));
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    config.attrs = attributes;
+    config.numAttrs = count;
+    return reported(cudaLaunchKernelEx(&config, kernel, static_cast<Parameters>(arguments)...));
+}
+
+template <typename... Parameters, typename... Arguments>
+cudaError_t launch(void (*kernel)(Parameters...), dim3 grid, int threads, size_t shared, cudaStream_t stream,
+                   Arguments... arguments) {
+    return launch_with(nullptr, 0, kernel, grid, threads, shared, stream, arguments...);
+}
+
 // Launches `kernel` behind the kernel in front of it on `stream` with
 // programmatic serialization: its CTAs may be resident before that kernel has
 // ended, and wait_for_previous() in it returns once all of that kernel's
@@ -48,14 +77,7 @@ cudaError_t launch_dependent(void (*kernel)(Parameters...), int grid, int thread
     cudaLaunchAttribute attribute{};
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(static_cast<unsigned>(grid));
-    config.blockDim = dim3(static_cast<unsigned>(threads));
-    config.dynamicSmemBytes = shared;
-    config.stream = stream;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, kernel, static_cast<Parameters>(arguments)...);
+    return launch_with(&attribute, 1, kernel, dim3(static_cast<unsigned>(grid)), threads, shared, stream, arguments...);
 }
 
 __device__ __forceinline__ void wait_for_previous() { cudaGridDependencySynchronize(); }

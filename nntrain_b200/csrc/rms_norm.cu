@@ -684,7 +684,7 @@ int resident_grid(int threads, int shared, long long rows) {
     std::atomic<int>& slot = known[threads / 32];
     int fit = slot.load(std::memory_order_relaxed);
     if (fit == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kKernel, threads, shared) != cudaSuccess || fit < 1)
+        if (reported(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kKernel, threads, shared)) != cudaSuccess || fit < 1)
             return grid_for(rows, 1);            // not kept: the next call asks again
         slot.store(fit, std::memory_order_relaxed);
     }
@@ -722,7 +722,7 @@ template <auto kKernel, int kThreadBytes>
 cudaError_t allow_shared() {
     constexpr int kMost = kStagedThreads * kThreadBytes;
     if constexpr (kMost < (40 << 10)) return cudaSuccess;
-    else return cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    else return reported(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
 }
 
 template <typename T, int kVec, int kGroups, int kBlock>
@@ -733,8 +733,7 @@ cudaError_t launch_forward(const ForwardArguments& a, int threads, cudaStream_t 
     const int shared = threads * kThreadBytes;
     const cudaError_t e = allow_shared<kKernel, kThreadBytes>();
     if (e != cudaSuccess) return e;
-    kKernel<<<resident_grid<kKernel>(threads, shared, a.rows), threads, shared, stream>>>(a);
-    return cudaPeekAtLastError();
+    return launch(kKernel, dim3(resident_grid<kKernel>(threads, shared, a.rows)), threads, shared, stream, a);
 }
 
 template <typename T, int kVec, int kGroups>
@@ -764,8 +763,7 @@ cudaError_t run_forward(const ForwardArguments& a, bool vector_ok, cudaStream_t 
         if (a.width <= 16 * kRowThreads) return forward_by_block<T, 1, 16>(a, threads_for(a.width, 16), stream);
     }
     constexpr auto kKernel = rms_norm_forward_loop_kernel<T>;
-    kKernel<<<resident_grid<kKernel>(kLoopThreads, 0, a.rows), kLoopThreads, 0, stream>>>(a);
-    return cudaPeekAtLastError();
+    return launch(kKernel, dim3(resident_grid<kKernel>(kLoopThreads, 0, a.rows)), kLoopThreads, 0, stream, a);
 }
 
 template <typename T, int kVec, int kGroups>
@@ -778,8 +776,7 @@ cudaError_t launch_backward(const BackwardArguments& a, int threads, int& grid, 
     if (e != cudaSuccess) return e;
     grid = resident_grid<kKernel>(threads, shared, a.rows);
     if (grid > kMostPartials) grid = kMostPartials;
-    kKernel<<<grid, threads, shared, stream>>>(a);
-    return cudaPeekAtLastError();
+    return launch(kKernel, dim3(grid), threads, shared, stream, a);
 }
 
 template <typename T>
@@ -796,8 +793,7 @@ cudaError_t run_backward(const BackwardArguments& a, bool vector_ok, int& grid, 
     constexpr auto kKernel = rms_norm_backward_loop_kernel<T>;
     grid = resident_grid<kKernel>(kLoopThreads, 0, a.rows);
     if (grid > kMostPartials) grid = kMostPartials;
-    kKernel<<<grid, kLoopThreads, 0, stream>>>(a);
-    return cudaPeekAtLastError();
+    return launch(kKernel, dim3(grid), kLoopThreads, 0, stream, a);
 }
 
 // Rows of `kind` at `p`, `stride` values apart: 128-bit accesses possible?

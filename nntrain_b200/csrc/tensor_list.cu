@@ -554,10 +554,7 @@ int clip_list(int device, const nntrain_gradient_tensor* tensors, int count, con
     const Chunk* chunks = reinterpret_cast<const Chunk*>(chunk_map);
     const int grid = static_cast<int>(chunk_count);
     cudaError_t e = cudaSuccess;
-    if (grid > 0) {
-        tensor_list_squares_kernel<<<grid, kThreads, 0, stream>>>(tensors, chunks, chunk_values, workspace);
-        e = cudaPeekAtLastError();
-    }
+    if (grid > 0) e = launch(tensor_list_squares_kernel, dim3(grid), kThreads, 0, stream, tensors, chunks, chunk_values, workspace);
     if (e != cudaSuccess) return static_cast<int>(e);
     const ClipArguments a{tensors, chunks, workspace, norm_and_coefficient, tensor_norms, finite_status, max_norm, count,
                           grid, chunk_values};

@@ -864,9 +864,8 @@ cudaError_t launch_lookup(const LookupArguments& a, bool vector_ok, cudaStream_t
     constexpr int kCtaTokens = kWarpsPerCta * kTokens;
     const dim3 grid(static_cast<unsigned>((a.count + kCtaTokens - 1) / kCtaTokens),
                     static_cast<unsigned>((a.width + kLookupColumns - 1) / kLookupColumns));
-    if (vector_ok) embedding_lookup_kernel<kTable, T, true, kTokens><<<grid, kThreads, 0, stream>>>(a);
-    else embedding_lookup_kernel<kTable, T, false, kTokens><<<grid, kThreads, 0, stream>>>(a);
-    return cudaPeekAtLastError();
+    return launch(vector_ok ? embedding_lookup_kernel<kTable, T, true, kTokens> : embedding_lookup_kernel<kTable, T, false, kTokens>,
+                  grid, kThreads, 0, stream, a);
 }
 
 // Four tokens a warp once that still leaves each SM 16 warps, else one.
@@ -956,12 +955,13 @@ cudaLaunchConfig_t cluster_launch(int cluster, long long ctas, int shared, cudaL
 template <int kCluster, int kResident>
 cudaError_t launch_cluster(SortKernel kernel, long long pieces, const SortArguments& a, cudaStream_t stream) {
     // the limit belongs to the device's context; setting it costs a fraction of a launch
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sort_shared<kCluster, kResident>());
+    const cudaError_t e =
+        reported(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sort_shared<kCluster, kResident>()));
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attribute{};
     const long long ctas = kCluster + (pieces + kCluster - 1) / kCluster * kCluster;
     const cudaLaunchConfig_t config = cluster_launch(kCluster, ctas, sort_shared<kCluster, kResident>(), attribute, stream);
-    return cudaLaunchKernelEx(&config, kernel, a);
+    return reported(cudaLaunchKernelEx(&config, kernel, a));
 }
 
 // Whether the current device runs clusters of 16 such CTAs: asked once per
@@ -999,11 +999,9 @@ cudaError_t launch_sort(SortArguments a, cudaStream_t stream) {
         int padded = 64;
         while (padded < static_cast<int>(a.count)) padded <<= 1;
         const unsigned ctas = static_cast<unsigned>(1 + pieces);
-        if (a.tokens.vocab < 1ll << (32 - kSmallBits))
-            embedding_small_sort_kernel<unsigned><<<ctas, kSortThreads, 0, stream>>>(a, padded);
-        else
-            embedding_small_sort_kernel<unsigned long long><<<ctas, kSortThreads, 0, stream>>>(a, padded);
-        return cudaPeekAtLastError();
+        return launch(a.tokens.vocab < 1ll << (32 - kSmallBits) ? embedding_small_sort_kernel<unsigned>
+                                                                : embedding_small_sort_kernel<unsigned long long>,
+                      dim3(ctas), kSortThreads, 0, stream, a, padded);
     }
     int bits = 1;                                // of the largest key, `vocab`
     while (a.tokens.vocab >> bits != 0) ++bits;
