@@ -308,8 +308,9 @@ int nntrain_gradient_clip_apply(int device, int kind, void* values, long long co
  * fp32 values (bf16: twice, BFP8: four times as long).  Call it with a null
  * chunk_map for the count, then with room for `capacity` chunks.  The first call
  * refuses a list in which what the clip writes for one tensor is read or written
- * for another one (a tensor twice, a destination over a neighbour); copy table and map to the device and use them for as long as
- * addresses and lengths stay what they are. */
+ * for another one (a tensor twice, a destination over a neighbour, scales over a
+ * payload); copy table and map to the device and use them for as long as addresses
+ * and lengths stay what they are. */
 int nntrain_gradient_list_plan(nntrain_gradient_tensor* tensors, int count, int* chunk_map,
                                long long capacity, long long* chunk_count, int* chunk_values);
 /* ABI minor 36.  The global norm over a list of tensors of mixed kinds and the
@@ -370,10 +371,11 @@ int nntrain_rms_norm_backward_workspace(long long rows, int width, long long* by
  * with g = dy * weight and n = h * i, x_gradient = i * (g - n * mean(g * n))
  * + residual_gradient, which is the gradient of x and of residual alike, and
  * weight_gradient = sum over rows of dy * n, added to what is there when
- * accumulate != 0.  residual_gradient (optional): the gradient that reaches h
- * from elsewhere.  x_gradient may be y_gradient or residual_gradient itself
- * when that is contiguous.  The scratch is the caller's, one for each call in
- * flight.  Fixed summation order: same inputs, same bits. */
+ * accumulate != 0; all in fp32, the sum over rows too.  residual_gradient
+ * (optional): the gradient that reaches h from elsewhere.  x_gradient may be
+ * y_gradient or residual_gradient itself when that is contiguous.  The scratch is
+ * the caller's, one for each call in flight.  Fixed summation order: same inputs,
+ * same bits. */
 int nntrain_rms_norm_backward(
     int device, int kind, const void* y_gradient, long long y_stride, const void* residual_gradient,
     long long residual_stride, const void* h, long long h_stride, const void* weight, int weight_kind,

@@ -49,6 +49,9 @@ enum Operation : std::uint32_t {
     kOpGradientPublishTensors = 216,
     // 217: the AdamW head that reads the encoded gradient (optimizer_head.cu)
     kOpGradientNorm = 218,
+    kOpTensorList = 219,
+    kOpRmsNorm = 220,
+    kOpTokenEmbedding = 221,
 };
 
 struct ErrorInfo {            // layout of nntrain_native_error_info (:74-82)

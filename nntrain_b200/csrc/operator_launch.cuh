@@ -8,10 +8,6 @@
 
 namespace ngb {
 
-constexpr Operation kOpTensorList = static_cast<Operation>(219);
-constexpr Operation kOpRmsNorm = static_cast<Operation>(220);
-constexpr Operation kOpTokenEmbedding = static_cast<Operation>(221);
-
 // A failed runtime call also stays behind as the thread's last error, where the
 // next check of any library in the process takes it for its own.  Here the entry
 // point's status tells it, so it is taken away.

@@ -21,10 +21,13 @@
 // registers are read again for each pass (they are in L1 / L2 then).
 //
 // Bound.  Backward: HBM, 8 bytes a value of bf16 with residual; 32768 x 1536 in
-// 69 us, 59 of them at 6.8 TB/s and the rest the join of the weight gradient.
+// 65 us, 59 of them at 6.8 TB/s and the rest the join of the weight gradient.
 // Forward: 7.1 bytes a value (x, residual, h, payload, scales; 2 more for a
 // decoded copy), but before that the instructions of the encode: 16384 x 1536
-// with the copy in 43 us, 75 % of the issue slots used, 82 % of HBM's rate.
+// with the copy in 41 us, 75 % of the issue slots used, 86 % of HBM's rate;
+// y alone, without an encode, in 38 us.  Narrow rows, one warp to a row, wait for
+// their two reductions instead: 2^20 x 128 bf16 without a residual 198 us forward
+// (2.7 TB/s) and 719 us backward, and half as wide ones take as long.
 #include "bfp8_kernels.cuh"
 #include "operator_launch.cuh"
 
@@ -700,8 +703,8 @@ int threads_for(int units, int groups) { return ((units + groups - 1) / groups +
 // Threads and groups per thread for a row of `units` groups of 8 values.  32
 // bytes of an input a thread (two groups of bf16, one of fp32) where there are
 // rows for all SMs, so that few warps share a row's barriers and its own
-// arithmetic (16384 x 1536 bf16: 43 us with 96 threads, 45 us with 192, 54 us
-// with 64; its gradient 69, 78 and 100 us for twice the rows), more where the row
+// arithmetic (16384 x 1536 bf16: 41 us with 96 threads, 43 us with 192, 58 us
+// with 64; its gradient 65, 72 and 140 us for twice the rows), more where the row
 // is longer than 256 threads then.
 template <typename T>
 RowShape row_shape(int units, long long rows) {
@@ -748,6 +751,13 @@ cudaError_t forward_by_block(const ForwardArguments& a, int threads, cudaStream_
     return cudaErrorInvalidValue;
 }
 
+// Rows in registers: blocks of 32, 64, 128 or the row on the 16-byte grid up to
+// 16384 values, blocks of 32 or the row off it up to 8192.  All else goes value by
+// value through memory: other blocks that divide the width, 64 and 128 off the grid,
+// longer rows.  It is right for all of them and several times slower (16384 x 1536
+// bf16 with residual: block 32 on the grid 38 us, off it 134 us; in the loop block 96
+// 162 us, 256 140 us, 64 off the grid 176 us; 2048 x 16384 in registers 55 us, 2048 x
+// 16416 in the loop 123 us).
 template <typename T>
 cudaError_t run_forward(const ForwardArguments& a, bool vector_ok, cudaStream_t stream) {
     const bool whole = a.payload == nullptr || a.block == a.width;
@@ -758,7 +768,7 @@ cudaError_t run_forward(const ForwardArguments& a, bool vector_ok, cudaStream_t 
         if (s.groups == 4) return forward_by_block<T, 8, 4>(a, s.threads, stream);
     } else if (whole || a.block == 32) {
         // 16 values a thread past one warp's: the barriers and the row's own arithmetic are shared by fewer warps
-        // (3001 x 771 fp32: 16.4 us with 4 or 8 values, 12.3 us with 16)
+        // (771 fp32, one scale a row: 3001 rows 11.7 us with 4 values, 10.3 us with 16, 10001 rows 32 and 26.5 us)
         if (a.width <= 512) return forward_by_block<T, 1, 4>(a, threads_for(a.width, 4), stream);
         if (a.width <= 16 * kRowThreads) return forward_by_block<T, 1, 16>(a, threads_for(a.width, 16), stream);
     }

@@ -44,9 +44,9 @@ constexpr int kFinishThreads = 1024;
 // A chunk is the same number of bytes for every kind: chunk_values fp32 values,
 // twice as many bf16 and four times as many BFP8 ones.  It grows with the list
 // (a 2048th of it) from 16 KB, one trip of a CTA, where a short list still
-// covers the SMs, to 96 KB.  Measured on the 41.6 M-value bf16 list: 52 us with
-// 16 KB chunks, 45 us with 48 KB, 47 us with 96 KB; on 1.54 G fp32 values 2.68 ms
-// with 96 KB and 2.71 ms with 256 KB.
+// covers the SMs, to 96 KB.  Measured on the 41.6 M-value bf16 list: 54 us with
+// 16 KB chunks, 45 us with 48 KB, 49 us with 96 KB; on 1.54 G fp32 values 2.93 ms
+// with 16 KB, 2.68 ms with 48 or 96 KB and 2.73 ms with 256 KB.
 constexpr long long kChunkLeast = 4096, kChunkMost = 24576;
 
 // Lists of at most this many chunks are finished by every CTA of the clip on

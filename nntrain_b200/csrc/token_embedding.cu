@@ -184,10 +184,11 @@ embedding_lookup_kernel(LookupArguments a) {
 constexpr int kSmallBits = 11, kSmallSort = 1 << kSmallBits;   // tokens that one CTA sorts
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 // CTAs of the sorting cluster: 8 is the portable size.  16, where the device has
-// them, for more tokens than one for each thread of 8 (20000 tokens added to a
-// table: 33 us with 8, 31 us with 16; 65536: 74 and 64 us), or beside zeros, which
-// clusters of 16 write more slowly, than 8 hold in their registers (30000 tokens
-// and 307 MB of zeros: 98 us with 8, 105 us with 16).
+// them, for more tokens than one for each thread of 8 (rows of 512 added to a
+// table: 8192 tokens 21.0 us with 8, 22.0 us with 16; 20000: 32.7 and 31.2 us;
+// 65536: 68 and 55 us), or beside zeros, which clusters of 16 write more slowly,
+// than 8 hold in their registers (30000 tokens and 307 MB of zeros: 84 us with 8,
+// 91 us with 16).
 constexpr int kClusterSmall = 8, kClusterLarge = 16;
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;   // of a pass at most
 constexpr int kLeastBits = 5;                   // a warp of digits
@@ -195,9 +196,9 @@ constexpr int kLeastBits = 5;                   // a warp of digits
 template <int kCluster, int kResident>
 constexpr int sort_shared() { return (kSortWarps * (kResident == 1 ? 2 : 1) + 2 + kCluster) * kDigits * 4; }
 // Zeros of a CTA beside the sort; and from how many bytes on, these and some for
-// each token, they take longer than the sort (8192 tokens, 197 MB: 59 us with two
-// CTAs of an SM, 61 us with one; 30000 tokens, 307 MB: 106 and 98 us; 65536
-// tokens, 98 MB: 98 and 83 us).
+// each token, they take longer than the sort (tables of 933 MB, 8192 tokens: 155 us
+// with two CTAs of an SM, 172 us with one; of 197 MB, 8192 tokens: 61.8 and 60.3 us;
+// of 307 MB, 30000 tokens: 98 and 84 us; of 98 MB, 65536 tokens: 119 and 102 us).
 constexpr long long kClearPiece = 128 << 10, kClearLong = 128ll << 20, kClearToken = 6 << 10;
 
 struct SortArguments {
@@ -369,8 +370,8 @@ __device__ __forceinline__ unsigned same_digit(bool here, unsigned digit, int bi
 // Stable: warps own consecutive stretches of the input, a warp walks its
 // stretch 32 at a time, and equal digits keep the order of their lanes.  A pair
 // is stored in one piece: the scattered stores of a few SMs, a 32-byte sector
-// each, are most of a pass over many tokens (65536 tokens, 8 CTAs: 47 us with
-// rows and positions apart, 35 us so).  A stretch that fits a warp's registers is
+// each, are most of a pass over many tokens (65536 tokens, 8 CTAs, all digits
+// ranked twice: 47 us with rows and positions apart, 35 us so).  A stretch that fits a warp's registers is
 // ranked once, when its digits are counted, and only placed afterwards.  Every CTA
 // writes its counts into the others' shared memory in front of the barrier that
 // it needs anyway, and sums them from its own.
@@ -525,9 +526,11 @@ embedding_sort_kernel(SortArguments a) {
 // ---- rows and join --------------------------------------------------------------
 
 // Sorted positions of a warp.  32, so that few tokens cross; 16 where 32 leave
-// the 148 SMs less than 64 warps of 256 columns each (added gradients: 65536
-// tokens x 512 72 us with 16, 74 us with 32, 76 us with 8; 131072 x 768 124, 120
-// and 141 us).
+// the 148 SMs less than 64 warps of 256 columns each (added gradients: 500 tokens x
+// 1536 13.5 us with 16, 18.1 us with 32; 16384 x 512 24.4 and 28.3 us; 131072 x 768
+// 148 and 138 us, 166 us with 8).  The border was measured when the join loaded
+// partials one after the other; now 32 would do a little better from about 4000
+// such warps on (65536 x 512 55.4 and 53.3 us).
 constexpr int kChunkMost = 32, kChunkLeast = 16;
 constexpr int kZeroRows = 32;                   // rows of a CTA that writes late zeros: one word of the bitmap
 // Columns of a warp: one 128-bit load of a lane, or 8 single values.
